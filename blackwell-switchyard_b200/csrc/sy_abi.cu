@@ -48,6 +48,15 @@ namespace sy {
 
 __device__ unsigned int g_device_error = 0;
 
+// Text of this thread's last CUDA error, for sy_status_string.
+static thread_local char t_last_error[256] = "";
+
+int cuda_error_status(cudaError_t e, const char* where) {
+  if (e == cudaSuccess) return SY_OK;
+  snprintf(t_last_error, sizeof(t_last_error), "%s: %s", where, cudaGetErrorString(e));
+  return SY_ERR_CUDA;
+}
+
 namespace {
 
 constexpr int64_t kMaxD = 1 << 24;  // D is converted to float exactly below 2^24
@@ -554,13 +563,7 @@ int64_t generic_partials(int64_t BT, const DevInfo& di) {
   return p < 1 ? 1 : p;
 }
 
-thread_local char t_last_error[256] = "";
 
-int cuda_status(cudaError_t e, const char* where) {
-  if (e == cudaSuccess) return SY_OK;
-  snprintf(t_last_error, sizeof(t_last_error), "%s: %s", where, cudaGetErrorString(e));
-  return SY_ERR_CUDA;
-}
 
 bool generic_fwd_fits(int64_t N, const DevInfo& di) {
   return N <= kGenericMaxN && (N * 8 * 2 + 3 * N) * 4 <= di.max_smem;
@@ -612,7 +615,7 @@ int sy_fwd(const void* v, const void* w, void* out, float* stats, int64_t N, int
   if (D > kMaxD || BT > INT_MAX) return SY_ERR_UNSUPPORTED;
   DevInfo di;
   cudaError_t e = dev_info(&di);
-  if (e != cudaSuccess) return cuda_status(e, "sy_fwd: device query");
+  if (e != cudaSuccess) return cuda_error_status(e, "sy_fwd: device query");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool aligned = al16(v) && al16(out);
   // The planners size kernels from the shape alone; eps is set here. Order:
@@ -622,26 +625,26 @@ int sy_fwd(const void* v, const void* w, void* out, float* stats, int64_t N, int
   sp.c.eps = eps;
   if (sp.ok && sp.c.reread && aligned) {
     e = launch_stream_fwd(sp.c, sp.grid, sp.cpl, dtype, v, w, w_dtype, out, stats, false, st);
-    return cuda_status(e, "sy_fwd: stream kernel launch");
+    return cuda_error_status(e, "sy_fwd: stream kernel launch");
   }
   TilePlan p = plan_tile(kOpFwd, N, BT, D, dtype, di);
   p.c.eps = eps;
   if (p.kind == kPlanRegTile && aligned) {
     e = launch_plan_fwd(p, dtype, v, w, w_dtype, out, stats, st);
-    return cuda_status(e, "sy_fwd: register-tile kernel launch");
+    return cuda_error_status(e, "sy_fwd: register-tile kernel launch");
   }
   if (sp.ok && aligned) {
     e = launch_stream_fwd(sp.c, sp.grid, sp.cpl, dtype, v, w, w_dtype, out, stats, false, st);
-    return cuda_status(e, "sy_fwd: stream kernel launch");
+    return cuda_error_status(e, "sy_fwd: stream kernel launch");
   }
   if (p.kind != kPlanGeneric && aligned) {
     e = launch_plan_fwd(p, dtype, v, w, w_dtype, out, stats, st);
-    return cuda_status(e, "sy_fwd: tile kernel launch");
+    return cuda_error_status(e, "sy_fwd: tile kernel launch");
   }
   if (!generic_fwd_fits(N, di)) return SY_ERR_UNSUPPORTED;
   e = launch_generic_fwd(BT, (int)N, (int)D, dtype, v, w, w_dtype, out, stats,
                          (int)stats_stride(N), eps, generic_grid(BT, di), st);
-  return cuda_status(e, "sy_fwd: generic kernel launch");
+  return cuda_error_status(e, "sy_fwd: generic kernel launch");
 }
 
 int64_t sy_bwd_partials(int64_t N, int64_t BT, int64_t D, int dtype) {
@@ -669,14 +672,14 @@ int sy_bwd(const void* v, const void* w, const void* g, const float* stats, void
   if (D == 0) return SY_OK;
   if (!dw_partial) return SY_ERR_ARG;
   if (BT == 0) {
-    return cuda_status(cudaMemsetAsync(dw_partial, 0, (size_t)P * D * sizeof(float), st),
+    return cuda_error_status(cudaMemsetAsync(dw_partial, 0, (size_t)P * D * sizeof(float), st),
                        "sy_bwd: zero dw_partial");
   }
   if (!v || !w || !g || !stats || !dv) return SY_ERR_ARG;
   if (D > kMaxD || BT > INT_MAX) return SY_ERR_UNSUPPORTED;
   DevInfo di;
   cudaError_t e = dev_info(&di);
-  if (e != cudaSuccess) return cuda_status(e, "sy_bwd: device query");
+  if (e != cudaSuccess) return cuda_error_status(e, "sy_bwd: device query");
   // Order: the register tile (N <= 16, rows up to 4 KiB), the row stream
   // (rows of 128 * K chunks, N <= 64), the shared-memory tile, generic.
   TilePlan p = plan_tile(kOpBwd, N, BT, D, dtype, di);
@@ -684,21 +687,21 @@ int sy_bwd(const void* v, const void* w, const void* g, const float* stats, void
   const bool aligned = al16(v) && al16(g) && al16(stats) && al16(dv) && al16(dw_partial);
   if (p.kind == kPlanRegTile && aligned) {
     e = launch_plan_bwd(p, dtype, v, w, w_dtype, g, stats, dv, dw_partial, st);
-    return cuda_status(e, "sy_bwd: register-tile kernel launch");
+    return cuda_error_status(e, "sy_bwd: register-tile kernel launch");
   }
   const StreamBwdPlan sb = plan_stream_bwd(N, BT, D, dtype, di);
   if (sb.ok && aligned) {
     e = launch_stream_bwd(sb.c, sb.grid, dtype, v, w, w_dtype, g, stats, dv, dw_partial, st);
-    return cuda_status(e, "sy_bwd: stream kernel launch");
+    return cuda_error_status(e, "sy_bwd: stream kernel launch");
   }
   if (p.kind != kPlanGeneric && aligned) {
     e = launch_plan_bwd(p, dtype, v, w, w_dtype, g, stats, dv, dw_partial, st);
-    return cuda_status(e, "sy_bwd: tile kernel launch");
+    return cuda_error_status(e, "sy_bwd: tile kernel launch");
   }
   if (N > kGenericMaxN || (N * 8 + 3 * N) * 4 > di.max_smem) return SY_ERR_UNSUPPORTED;
   e = launch_generic_bwd(BT, (int)N, (int)D, dtype, v, w, w_dtype, g, stats, (int)stats_stride(N),
                          dv, dw_partial, (int)P, eps, st);
-  return cuda_status(e, "sy_bwd: generic kernel launch");
+  return cuda_error_status(e, "sy_bwd: generic kernel launch");
 }
 
 int sy_dw_reduce(const float* dw_partial, int64_t P, int64_t D, void* dw, int dw_dtype,
@@ -711,7 +714,7 @@ int sy_dw_reduce(const float* dw_partial, int64_t P, int64_t D, void* dw, int dw
   const cudaError_t e =
       launch_dw_reduce(dw_partial, P, D, dw, dw_dtype, SY_TUNE_PDL != 0,
                        static_cast<cudaStream_t>(stream));
-  return cuda_status(e, "sy_dw_reduce: launch");
+  return cuda_error_status(e, "sy_dw_reduce: launch");
 }
 
 int sy_dw_reduce_gain(const float* dw_partial, int64_t P, int64_t D, const void* w, const void* g,
@@ -724,7 +727,7 @@ int sy_dw_reduce_gain(const float* dw_partial, int64_t P, int64_t D, const void*
   const cudaError_t e =
       launch_dw_reduce(dw_partial, P, D, dw, wg_dtype, SY_TUNE_PDL != 0,
                        static_cast<cudaStream_t>(stream), w, g, dg);
-  return cuda_status(e, "sy_dw_reduce_gain: launch");
+  return cuda_error_status(e, "sy_dw_reduce_gain: launch");
 }
 
 int sy_fwd_batched(const void* v, const void* queries, void* out, int64_t N, int64_t BT, int64_t D,
@@ -737,24 +740,24 @@ int sy_fwd_batched(const void* v, const void* queries, void* out, int64_t N, int
   if (S == 1) return sy_fwd(v, queries, out, nullptr, N, BT, D, dtype, dtype, eps, stream);
   DevInfo di;
   cudaError_t e = dev_info(&di);
-  if (e != cudaSuccess) return cuda_status(e, "sy_fwd_batched: device query");
+  if (e != cudaSuccess) return cuda_error_status(e, "sy_fwd_batched: device query");
   TilePlan bp = plan_batched(N, BT, D, S, dtype, di);
   bp.c.eps = eps;
   if (bp.kind == kPlanRegTile && al16(v) && al16(queries) && al16(out)) {
     e = launch_plan_batched(bp, (int)S, dtype, v, queries, out, static_cast<cudaStream_t>(stream));
-    return cuda_status(e, "sy_fwd_batched: register-tile kernel launch");
+    return cuda_error_status(e, "sy_fwd_batched: register-tile kernel launch");
   }
   StreamBatchedPlan sb = plan_stream_batched(N, BT, D, S, dtype, di);
   sb.c.eps = eps;
   if (sb.ok && al16(v) && al16(queries) && al16(out)) {
     e = launch_stream_batched(sb.c, sb.grid, dtype, v, queries, out,
                               static_cast<cudaStream_t>(stream));
-    return cuda_status(e, "sy_fwd_batched: stream kernel launch");
+    return cuda_error_status(e, "sy_fwd_batched: stream kernel launch");
   }
   if (!generic_batched_fits(N, S, di)) return SY_ERR_UNSUPPORTED;
   e = launch_generic_batched(BT, (int)N, (int)D, (int)S, dtype, nullptr, 0, v, queries, out, eps,
                              generic_grid(BT, di), static_cast<cudaStream_t>(stream));
-  return cuda_status(e, "sy_fwd_batched: generic kernel launch");
+  return cuda_error_status(e, "sy_fwd_batched: generic kernel launch");
 }
 
 int sy_fwd_batched_stats(const void* v, const void* queries, void* out, float* mstats, int raw,
@@ -768,7 +771,7 @@ int sy_fwd_batched_stats(const void* v, const void* queries, void* out, float* m
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   DevInfo di;
   cudaError_t e = dev_info(&di);
-  if (e != cudaSuccess) return cuda_status(e, "sy_fwd_batched_stats: device query");
+  if (e != cudaSuccess) return cuda_error_status(e, "sy_fwd_batched_stats: device query");
   const bool aligned = al16(v) && al16(queries) && al16(out) && al8(mstats);
   TilePlan bp = plan_batched(N, BT, D, S, dtype, di);
   bp.c.eps = eps;
@@ -776,7 +779,7 @@ int sy_fwd_batched_stats(const void* v, const void* queries, void* out, float* m
   bp.c.raw = raw;
   if (bp.kind == kPlanRegTile && aligned) {
     e = launch_plan_batched(bp, (int)S, dtype, v, queries, out, st);
-    return cuda_status(e, "sy_fwd_batched_stats: register-tile kernel launch");
+    return cuda_error_status(e, "sy_fwd_batched_stats: register-tile kernel launch");
   }
   StreamBatchedPlan sb = plan_stream_batched(N, BT, D, S, dtype, di);
   sb.c.eps = eps;
@@ -784,12 +787,12 @@ int sy_fwd_batched_stats(const void* v, const void* queries, void* out, float* m
   sb.c.raw = raw;
   if (sb.ok && aligned) {
     e = launch_stream_batched(sb.c, sb.grid, dtype, v, queries, out, st);
-    return cuda_status(e, "sy_fwd_batched_stats: stream kernel launch");
+    return cuda_error_status(e, "sy_fwd_batched_stats: stream kernel launch");
   }
   if (!generic_batched_fits(N, S, di) || !al8(mstats)) return SY_ERR_UNSUPPORTED;
   e = launch_generic_batched(BT, (int)N, (int)D, (int)S, dtype, mstats, raw, v, queries, out, eps,
                              generic_grid(BT, di), st);
-  return cuda_status(e, "sy_fwd_batched_stats: generic kernel launch");
+  return cuda_error_status(e, "sy_fwd_batched_stats: generic kernel launch");
 }
 
 int64_t sy_bwd_batched_partials(int64_t N, int64_t BT, int64_t D, int64_t S, int dtype) {
@@ -814,24 +817,24 @@ int sy_bwd_batched(const void* v, const void* queries, const void* g, void* dv,
   if (D == 0) return SY_OK;
   if (!dq_partial) return SY_ERR_ARG;
   if (BT == 0)
-    return cuda_status(cudaMemsetAsync(dq_partial, 0, (size_t)P * S * D * sizeof(float), st),
+    return cuda_error_status(cudaMemsetAsync(dq_partial, 0, (size_t)P * S * D * sizeof(float), st),
                        "sy_bwd_batched: zero dq_partial");
   if (!v || !queries || !g || !dv) return SY_ERR_ARG;
   if (S > 16) return SY_ERR_UNSUPPORTED;
   if (D > kMaxD || BT > INT_MAX) return SY_ERR_UNSUPPORTED;
   DevInfo di;
   cudaError_t e = dev_info(&di);
-  if (e != cudaSuccess) return cuda_status(e, "sy_bwd_batched: device query");
+  if (e != cudaSuccess) return cuda_error_status(e, "sy_bwd_batched: device query");
   const int variant = reg_bwd_batched_variant((int)N, (int)D, (int)S, dtype, di.max_smem);
   if (variant > 0 && al16(v) && al16(queries) && al16(g) && al16(dv) && al16(dq_partial)) {
     e = launch_reg_bwd_batched(BT, (int)N, (int)D, (int)S, dtype, v, queries, g, dv, dq_partial,
                                (int)P, eps, variant, st);
-    return cuda_status(e, "sy_bwd_batched: register-tile kernel launch");
+    return cuda_error_status(e, "sy_bwd_batched: register-tile kernel launch");
   }
   if (bwd_batched_smem((int)N, (int)S) > (size_t)di.max_smem) return SY_ERR_UNSUPPORTED;
   e = launch_bwd_batched(BT, (int)N, (int)D, (int)S, dtype, v, queries, g, dv, dq_partial, (int)P,
                          eps, st);
-  return cuda_status(e, "sy_bwd_batched: kernel launch");
+  return cuda_error_status(e, "sy_bwd_batched: kernel launch");
 }
 
 int sy_stage_partial(const void* partial, const void* out, void* new_partial, void* arena_slot,
@@ -842,7 +845,7 @@ int sy_stage_partial(const void* partial, const void* out, void* new_partial, vo
   if (!partial || !out || !arena_slot) return SY_ERR_ARG;
   DevInfo di;
   cudaError_t e = dev_info(&di);
-  if (e != cudaSuccess) return cuda_status(e, "sy_stage_partial: device query");
+  if (e != cudaSuccess) return cuda_error_status(e, "sy_stage_partial: device query");
   const int es = esize_of(dtype);
   const bool vec16 = (numel * es) % 16 == 0 && al16(partial) && al16(out) && al16(arena_slot) &&
                      (new_partial == nullptr || al16(new_partial));
@@ -851,7 +854,7 @@ int sy_stage_partial(const void* partial, const void* out, void* new_partial, vo
   const int64_t blocks = (work + 255) / 256;
   e = launch_stage(numel, dtype, partial, out, new_partial, arena_slot, vec16,
                    (int)(blocks < cap ? blocks : cap), static_cast<cudaStream_t>(stream));
-  return cuda_status(e, "sy_stage_partial: kernel launch");
+  return cuda_error_status(e, "sy_stage_partial: kernel launch");
 }
 
 int sy_merge_stats(const void* o1, const float* ms1, const void* o2, const float* ms2, void* o,
@@ -865,12 +868,12 @@ int sy_merge_stats(const void* o1, const float* ms1, const void* o2, const float
   if (D > kMaxD) return SY_ERR_UNSUPPORTED;
   DevInfo di;
   cudaError_t e = dev_info(&di);
-  if (e != cudaSuccess) return cuda_status(e, "sy_merge_stats: device query");
+  if (e != cudaSuccess) return cuda_error_status(e, "sy_merge_stats: device query");
   const int vec16 = (D * esize_of(dtype)) % 16 == 0 && al16(o1) && al16(o2) && al16(o);
   const int64_t cap = (int64_t)di.sms * 8;  // one row per CTA, 8 CTAs per SM in flight
   e = launch_merge(R, (int)D, dtype, o1, ms1, o2, ms2, o, ms, normalize, vec16,
                    (int)(R < cap ? R : cap), static_cast<cudaStream_t>(stream));
-  return cuda_status(e, "sy_merge_stats: kernel launch");
+  return cuda_error_status(e, "sy_merge_stats: kernel launch");
 }
 
 int sy_speed_of_light(const void* v, void* out, int64_t N, int64_t BT, int64_t D, int dtype,
@@ -882,20 +885,20 @@ int sy_speed_of_light(const void* v, void* out, int64_t N, int64_t BT, int64_t D
   if (D > kMaxD || BT > INT_MAX) return SY_ERR_UNSUPPORTED;
   DevInfo di;
   cudaError_t e = dev_info(&di);
-  if (e != cudaSuccess) return cuda_status(e, "sy_speed_of_light: device query");
+  if (e != cudaSuccess) return cuda_error_status(e, "sy_speed_of_light: device query");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const StreamPlan sp = plan_stream(N, BT, D, dtype, di, /*sol=*/true);
   if (sp.ok && al16(v) && al16(out)) {
     e = launch_stream_fwd(sp.c, sp.grid, sp.cpl, dtype, v, nullptr, SY_F32, out, nullptr, true, st);
-    return cuda_status(e, "sy_speed_of_light: stream kernel launch");
+    return cuda_error_status(e, "sy_speed_of_light: stream kernel launch");
   }
   const TilePlan p = plan_tile(kOpSol, N, BT, D, dtype, di);
   if (p.kind != kPlanGeneric && al16(v) && al16(out)) {
     e = launch_tile_sol(p.c, p.grid, p.cpt, dtype, v, out, st);
-    return cuda_status(e, "sy_speed_of_light: tile kernel launch");
+    return cuda_error_status(e, "sy_speed_of_light: tile kernel launch");
   }
   e = launch_generic_sol(BT, (int)N, (int)D, dtype, v, out, generic_grid(BT, di), st);
-  return cuda_status(e, "sy_speed_of_light: generic kernel launch");
+  return cuda_error_status(e, "sy_speed_of_light: generic kernel launch");
 }
 
 int sy_plan_info(int op, int64_t N, int64_t BT, int64_t D, int64_t S, int dtype, int sms,
@@ -910,7 +913,7 @@ int sy_plan_info(int op, int64_t N, int64_t BT, int64_t D, int64_t S, int dtype,
     di.l2 = kAssumedL2Bytes;
   } else {
     const cudaError_t e = dev_info(&di);
-    if (e != cudaSuccess) return cuda_status(e, "sy_plan_info: device query");
+    if (e != cudaSuccess) return cuda_error_status(e, "sy_plan_info: device query");
   }
   const int64_t bt = BT < 1 ? 1 : BT;
   int top = op == 1 ? kOpBwd : (op == 3 ? kOpSol : kOpFwd);
@@ -985,13 +988,13 @@ int sy_plan_kind(int op, int64_t N, int64_t BT, int64_t D, int64_t S, int dtype)
 int sy_device_error(int* code) {
   if (!code) return SY_ERR_ARG;
   cudaError_t e = cudaDeviceSynchronize();
-  if (e != cudaSuccess) return cuda_status(e, "sy_device_error: synchronize");
+  if (e != cudaSuccess) return cuda_error_status(e, "sy_device_error: synchronize");
   unsigned int v = 0;
   e = cudaMemcpyFromSymbol(&v, g_device_error, sizeof(v));
-  if (e != cudaSuccess) return cuda_status(e, "sy_device_error: read");
+  if (e != cudaSuccess) return cuda_error_status(e, "sy_device_error: read");
   const unsigned int zero = 0;
   e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof(zero));
-  if (e != cudaSuccess) return cuda_status(e, "sy_device_error: clear");
+  if (e != cudaSuccess) return cuda_error_status(e, "sy_device_error: clear");
   *code = (int)v;
   return SY_OK;
 }

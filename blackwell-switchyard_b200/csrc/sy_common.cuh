@@ -20,7 +20,7 @@ namespace sy {
 // ---------------------------------------------------------------------------
 // Device error word. Bit flags; read and cleared by sy_device_error().
 // ---------------------------------------------------------------------------
-enum : unsigned { kDevErrWaitTimeout = 1u, kDevErrBadPlan = 2u };
+enum : unsigned { kDevErrWaitTimeout = 1u, kDevErrBadPlan = 2u, kDevErrBadIndex = 4u };
 extern __device__ unsigned int g_device_error;
 
 // A legitimate wait in these kernels lasts microseconds (one HBM round trip

@@ -9,6 +9,9 @@
 
 namespace sy {
 
+// SY_OK, or SY_ERR_CUDA with the error's text kept for sy_status_string.
+int cuda_error_status(cudaError_t e, const char* where);
+
 // Raise a kernel's dynamic shared-memory limit once per (kernel, device).
 template <typename... KArgs>
 cudaError_t raise_smem_limit(void (*kern)(KArgs...), size_t smem) {

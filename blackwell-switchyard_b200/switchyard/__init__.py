@@ -15,6 +15,7 @@ from .triton_op import (
     speed_of_light,
 )
 from .arena import stage_partial
+from .serving import append_kv, attend_paged, sample_tokens
 from .two_phase import attn_with_stats, block_attn_res_batched_train, merge_online_softmax
 
 __version__ = "0.1.0"
@@ -30,4 +31,7 @@ __all__ = [
     "merge_online_softmax",
     "block_attn_res_batched_train",
     "stage_partial",
+    "append_kv",
+    "attend_paged",
+    "sample_tokens",
 ]

@@ -52,6 +52,12 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "sy_dw_exchange": ([_P, _I64, _I64, _P, _I, _I, _I64, _c.c_uint32, _P, _I,
                         _c.c_uint64, _P, _P, _P], _I),
     "sy_dw_exchange_bytes": ([_I64, _I], _I64),
+    # serving: argument structs by address (the extension fills them)
+    "sy_append_kv": ([_P, _P], _I),
+    "sy_attend_workspace": ([_P], _I64),
+    "sy_attend": ([_P, _P], _I),
+    "sy_sample_workspace": ([_P], _I64),
+    "sy_sample": ([_P, _P], _I),
 }
 
 

@@ -293,10 +293,123 @@ SY_API int sy_dw_exchange(const float* dw_partial, int64_t P, int64_t L,
 SY_API int64_t sy_dw_exchange_bytes(int64_t L, int world);
 
 /*
+ * ---------------------------------------------------------------------------
+ * Serving: a paged key/value cache, attention over it, and sampling
+ * ---------------------------------------------------------------------------
+ * No reference counterpart: the reference trains and has no cache. These three
+ * let the decoder that calls the operator continue a prompt.
+ *
+ * A cache is [pages, kv_heads, page_size, head_dim] for keys and the same for
+ * values, any strides whose last one is 1 (element strides below). Slot s is
+ * row s % page_size of page s / page_size. Indices that come from device
+ * memory (slots, positions, page numbers, lengths) are checked by the kernels:
+ * one outside its buffer is not followed and sets bit 4 of the device error
+ * word (sy_device_error).
+ */
+typedef struct sy_append_kv_args {
+  const void* q; /* [tokens, q_heads, head_dim] or NULL (q_heads 0) */
+  const void* k; /* [tokens, kv_heads, head_dim] */
+  const void* v; /* [tokens, kv_heads, head_dim] */
+  void* q_out;   /* [tokens, q_heads, head_dim], contiguous; NULL without q */
+  void* k_cache;
+  void* v_cache;
+  const int64_t* slots;     /* [tokens]; negative: the token is not written */
+  const int32_t* positions; /* [tokens] rows of cos/sin; NULL: no rotation */
+  const float* cos;         /* [rope_len, rot_half] fp32, rows rope_row apart */
+  const float* sin;
+  int64_t tokens, q_heads, kv_heads, head_dim;
+  int64_t rot_half, rope_len, rope_row;
+  int64_t pages, page_size;
+  int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;
+  int64_t kc_page, kc_head, kc_row, vc_page, vc_head, vc_row;
+  int32_t dtype;
+} sy_append_kv_args;
+
+/*
+ * Rotate and append. With h = rot_half and (c, s) = (cos, sin)[position]:
+ *   y[i] = x[i] c[i] - x[i+h] s[i],  y[i+h] = x[i+h] c[i] + x[i] s[i],  i < h,
+ *   y[i] = x[i] for i >= 2h
+ * in fp32 with one rounding. q_out = rotated q; the rotated k and the v of
+ * every token with slot >= 0 are written to their rows of the caches. Two live
+ * tokens with one slot race. One launch.
+ */
+SY_API int sy_append_kv(const sy_append_kv_args* args, sy_stream_t stream);
+
+typedef struct sy_attend_args {
+  const void* q; /* [batch, q_len, q_heads, head_dim] */
+  const void* k_cache;
+  const void* v_cache;
+  void* out;                   /* [batch, q_len, q_heads, head_dim], contiguous */
+  float* lse;                  /* [batch, q_len, q_heads] or NULL */
+  const int32_t* page_table;   /* [batch, table_width], rows table_row apart */
+  const int32_t* kv_lens;      /* [batch] */
+  const int32_t* prefix_pages; /* [ceil(prefix_len / page_size)] */
+  void* workspace;             /* sy_attend_workspace bytes, 16-byte aligned */
+  int64_t workspace_bytes;
+  int64_t batch, q_len, q_heads, kv_heads, head_dim;
+  int64_t pages, page_size, table_width, table_row, prefix_len;
+  int64_t q_b, q_t, q_h;
+  int64_t kc_page, kc_head, kc_row, vc_page, vc_head, vc_row;
+  float scale;
+  int32_t dtype; /* SY_BF16 or SY_F16 */
+} sy_attend_args;
+
+/* Bytes of workspace sy_attend needs for these sizes (pointers are not read),
+ * or -status. */
+SY_API int64_t sy_attend_workspace(const sy_attend_args* args);
+
+/*
+ * Attention of every sequence's last q_len tokens over the prefix that the
+ * whole batch shares and over the sequence's own keys. Query t of sequence b
+ * sees prefix keys 0..prefix_len-1 and own keys j < kv_lens[b] - q_len + t + 1:
+ *   out = sum_j softmax_j(scale q.k_j) v_j,   lse = log sum_j exp(scale q.k_j)
+ * A query that sees no key gets out = 0 and lse = -inf. Query head h reads key
+ * head h / (q_heads / kv_heads). Own key j is row j % page_size of page
+ * page_table[b, j / page_size]; entries past a sequence's length are not read.
+ * Rows of a page past the length may hold anything, NaN included. head_dim is
+ * a multiple of 8 up to 128 and page_size a multiple of 8; pointers and strides
+ * (in bytes) are multiples of 16.
+ */
+SY_API int sy_attend(const sy_attend_args* args, sy_stream_t stream);
+
+typedef struct sy_sample_args {
+  const void* logits;       /* [rows, vocab], rows logits_row apart */
+  const float* u;           /* [rows] in [0, 1) */
+  const float* temperature; /* [rows] or NULL (1) */
+  const int32_t* top_k;     /* [rows] or NULL (off); <= 0 is off */
+  const float* top_p;       /* [rows] or NULL (off); >= 1 is off */
+  const float* min_p;       /* [rows] or NULL (off); <= 0 is off */
+  int64_t* token;           /* [rows] */
+  float* logprob;           /* [rows] or NULL */
+  void* workspace;          /* sy_sample_workspace bytes, 16-byte aligned, or NULL if 0 */
+  int64_t workspace_bytes;
+  int64_t rows, vocab, logits_row;
+  int32_t dtype;
+} sy_sample_args;
+
+/* Bytes of workspace sy_sample needs for these sizes, or -status. */
+SY_API int64_t sy_sample_workspace(const sy_sample_args* args);
+
+/*
+ * One token a row. x = logit * (1 / temperature) in fp32, NaN counted as -inf;
+ * weights are whole numbers w_i = rint(2^40 exp(x_i - max x)), so that every
+ * sum below is exact and no order of summation shows in the result. Tokens are
+ * ranked by x, highest first, ties by index. Kept are the first top_k; of
+ * those with total weight Z the ranks whose preceding weight is below
+ * ceil(top_p Z), the first always; of those the ones with exp(x_i - max x) >=
+ * min(min_p, 1). The token is the first in index order whose inclusive kept
+ * weight exceeds floor(u Z_kept); logprob = log(w_token / Z_kept).
+ * temperature <= 0 takes the highest logit. A row without a logit above -inf
+ * gives token -1 and logprob NaN.
+ */
+SY_API int sy_sample(const sy_sample_args* args, sy_stream_t stream);
+
+/*
  * Reads the device-side error word of the current device and clears it.
  * Synchronises the device. Bit 1: a kernel's bounded wait ran out; bit 2: a
- * kernel refused an inconsistent launch plan. Writes 0 to *code when no error
- * was recorded.
+ * kernel refused an inconsistent launch plan; bit 4: an index in device memory
+ * (a slot, position, page number or length) was outside its buffer and was not
+ * followed. Writes 0 to *code when no error was recorded.
  */
 SY_API int sy_device_error(int* code);
 
