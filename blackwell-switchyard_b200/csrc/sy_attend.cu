@@ -301,7 +301,7 @@ __device__ __forceinline__ bool load_queries(const Plan& p, char* smem, Bars* ba
 struct MmaState {
   int pos = 0;         // ring position of the phase's first tile
   int slot = 0;        // query slots used by S so far
-  int p_count[2] = {0, 0};
+  uint32_t p_phase = 0;  // bit s: parity of stream s's next P
 };
 
 template <int DP, bool BF16, bool Pre>
@@ -364,8 +364,8 @@ __device__ __forceinline__ bool issue_mmas(const Plan& p, char* smem, Bars* bars
     }
     const uint64_t b = sw128_desc(base + S::kRing + stage * S::kTileBytes, kTile * 128, 1024);
     for (int s = wide ? 0 : cur.j & 1; s <= (wide ? 1 : cur.j & 1); ++s) {
-      SY_WAIT(&bars->p_full[s], st.p_count[s] & 1);
-      ++st.p_count[s];
+      SY_WAIT(&bars->p_full[s], (st.p_phase >> s) & 1);
+      st.p_phase ^= 1u << s;
       tc_fence_after();
       const int step = wide ? 1 : 2;  // tiles between two of this stream
       if (lane == 0) {
@@ -410,6 +410,21 @@ __device__ __forceinline__ constexpr float weight_shift() {
   return sizeof(T) == 2 && std::is_same<T, __half>::value ? 6.f : 0.f;
 }
 
+__device__ __forceinline__ void mask_columns(uint32_t* x, int upto) {
+#pragma unroll
+  for (int k = 0; k < 32; ++k)
+    if (k >= upto) x[k] = 0xff800000u;  // -inf
+}
+__device__ __forceinline__ float row_max(const uint32_t* x) {
+  float a = __uint_as_float(x[0]), b = __uint_as_float(x[1]);
+#pragma unroll
+  for (int k = 2; k < 32; k += 2) {
+    a = fmaxf(a, __uint_as_float(x[k]));
+    b = fmaxf(b, __uint_as_float(x[k + 1]));
+  }
+  return fmaxf(a, b);
+}
+
 template <typename T, int DP, bool Pre>
 __device__ __forceinline__ bool softmax_tiles(const Plan& p, Bars* bars, uint32_t tmem, int s,
                                               Cursor<Pre> cur, bool wide, const Part& part,
@@ -437,24 +452,22 @@ __device__ __forceinline__ bool softmax_tiles(const Plan& p, Bars* bars, uint32_
     ++st.s_count;
     tc_fence_after();
     if (warp * 32 < rows) {
-      uint32_t x[kTile];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) tmem_ld32(s_at + 32 * i, x + 32 * i);
-      tmem_wait_ld();
+      // The row is read twice, 32 columns at a time: held whole it would take
+      // every register of the thread.
+      uint32_t xa[32], xb[32];
+      tmem_ld32(s_at, xa);
       const int keys = cur.keys(p);
       const int upto = cur.in_prefix(p) ? keys : min(keys, see - cur.key0(p));
-      if (__any_sync(kFull, upto < kTile)) {
+      const bool masked = __any_sync(kFull, upto < kTile);
+      float top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < kTile; ++i)
-          if (i >= upto) x[i] = 0xff800000u;  // -inf
+      for (int i = 0; i < 4; ++i) {
+        uint32_t* x = i & 1 ? xb : xa;
+        tmem_wait_ld(x);
+        if (i < 3) tmem_ld32(s_at + 32 * (i + 1), i & 1 ? xa : xb);
+        if (masked) mask_columns(x, upto - 32 * i);
+        top = fmaxf(top, row_max(x));
       }
-      float top0 = __uint_as_float(x[0]), top1 = __uint_as_float(x[1]);
-#pragma unroll
-      for (int i = 2; i < kTile; i += 2) {
-        top0 = fmaxf(top0, __uint_as_float(x[i]));
-        top1 = fmaxf(top1, __uint_as_float(x[i + 1]));
-      }
-      const float top = fmaxf(top0, top1);
       // The first maximum is taken as it is; later ones only past 2^kGrow.
       const bool moves = m == -INFINITY ? top > -INFINITY : (top - m) * c > kGrow;
       if (__any_sync(kFull, moves)) {
@@ -467,7 +480,7 @@ __device__ __forceinline__ bool softmax_tiles(const Plan& p, Bars* bars, uint32_
           for (int i = 0; i < DP / 32; ++i) {
             uint32_t o[32];
             tmem_ld32(o_at + 32 * i, o);
-            tmem_wait_ld();
+            tmem_wait_ld(o);
 #pragma unroll
             for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
             tmem_st32(o_at + 32 * i, o);
@@ -477,22 +490,30 @@ __device__ __forceinline__ bool softmax_tiles(const Plan& p, Bars* bars, uint32_
       const float off = (m == -INFINITY ? 0.f : -m * c) + weight_shift<T>();
       const float2 c2 = make_float2(c, c), off2 = make_float2(off, off);
       float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
+      tmem_ld32(s_at, xa);
 #pragma unroll
-      for (int i = 0; i < kTile; i += 4) {
-        float2 u = make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1]));
-        float2 w = make_float2(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
-        u = __ffma2_rn(u, c2, off2);
-        w = __ffma2_rn(w, c2, off2);
-        u = make_float2(ex2(u.x), ex2(u.y));
-        w = make_float2(ex2(w.x), ex2(w.y));
-        sum0 = __fadd2_rn(sum0, u);
-        sum1 = __fadd2_rn(sum1, w);
-        x[i / 2] = pack16<T>(u.x, u.y);
-        x[i / 2 + 1] = pack16<T>(w.x, w.y);
+      for (int i = 0; i < 4; ++i) {
+        uint32_t* x = i & 1 ? xb : xa;
+        tmem_wait_ld(x);
+        if (i < 3) tmem_ld32(s_at + 32 * (i + 1), i & 1 ? xa : xb);
+        if (masked) mask_columns(x, upto - 32 * i);
+#pragma unroll
+        for (int k = 0; k < 32; k += 4) {
+          float2 u = make_float2(__uint_as_float(x[k]), __uint_as_float(x[k + 1]));
+          float2 w = make_float2(__uint_as_float(x[k + 2]), __uint_as_float(x[k + 3]));
+          u = __ffma2_rn(u, c2, off2);
+          w = __ffma2_rn(w, c2, off2);
+          u = make_float2(ex2(u.x), ex2(u.y));
+          w = make_float2(ex2(w.x), ex2(w.y));
+          sum0 = __fadd2_rn(sum0, u);
+          sum1 = __fadd2_rn(sum1, w);
+          x[k / 2] = pack16<T>(u.x, u.y);
+          x[k / 2 + 1] = pack16<T>(w.x, w.y);
+        }
+        // P takes half of S's columns: these 16 were read in this step or before
+        tmem_st16(s_at + 16 * i, x);
       }
       l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
-      tmem_st32(s_at, x);
-      tmem_st32(s_at + 32, x + 32);
       tmem_wait_st();
     }
     tc_fence_before();
@@ -526,7 +547,7 @@ __device__ __forceinline__ bool softmax_tiles(const Plan& p, Bars* bars, uint32_
         for (int i = 0; i < DP / 32; ++i) {
           uint32_t o[32];
           tmem_ld32(o_at + 32 * i, o);
-          tmem_wait_ld();
+          tmem_wait_ld(o);
           if (!final) {
 #pragma unroll
             for (int k = 0; k < 32; k += 4)

@@ -43,7 +43,6 @@ __device__ __forceinline__ void tc_commit(uint64_t* bar) {
 // TMEM <-> registers: 32 lanes x 32 bit, 32 columns (lane = row of the warp's
 // quarter of TMEM, register i = column i)
 // ---------------------------------------------------------------------------
-#define SY_R8(a, i) a[i], a[i + 1], a[i + 2], a[i + 3], a[i + 4], a[i + 5], a[i + 6], a[i + 7]
 #define SY_OUT4(a, i) "=r"(a[i]), "=r"(a[i + 1]), "=r"(a[i + 2]), "=r"(a[i + 3])
 #define SY_IN4(a, i) "r"(a[i]), "r"(a[i + 1]), "r"(a[i + 2]), "r"(a[i + 3])
 
@@ -65,8 +64,22 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
       SY_IN4(r, 24), SY_IN4(r, 28)
       : "memory");
 }
-__device__ __forceinline__ void tmem_wait_ld() {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+      SY_IN4(r, 0), SY_IN4(r, 4), SY_IN4(r, 8), SY_IN4(r, 12)
+      : "memory");
+}
+// Wait for this thread's TMEM loads. The 32 registers of the last one pass
+// through, so that nothing that uses them is scheduled before the wait.
+#define SY_IO4(a, i) "+r"(a[i]), "+r"(a[i + 1]), "+r"(a[i + 2]), "+r"(a[i + 3])
+__device__ __forceinline__ void tmem_wait_ld(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : SY_IO4(r, 0), SY_IO4(r, 4), SY_IO4(r, 8), SY_IO4(r, 12), SY_IO4(r, 16),
+                 SY_IO4(r, 20), SY_IO4(r, 24), SY_IO4(r, 28)
+               :
+               : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
