@@ -39,6 +39,7 @@ namespace {
 
 constexpr int kTile = 128;     // keys of a tile, rows of a stream
 constexpr int kThreads = 384;  // load, MMA, 2 query warps, 2 x 4 softmax warps
+constexpr int kBarBytes = 3072;  // barriers and scratch behind the tiles
 constexpr float kGrow = 8.f;   // log2 of the growth of a maximum that is let pass
 
 struct Plan {
@@ -78,6 +79,22 @@ __device__ __forceinline__ int entry_limit(const Plan& p, int row_tile, int len)
 __device__ __forceinline__ int entry_tiles(const Plan& p, int lim) {
   return p.lead_tiles + (lim + kTile - 1) / kTile;
 }
+
+// The line's cut: CTA c has the tiles [first(c), first(c + 1)).
+struct Cut {
+  long long total;
+  int grid;
+  long long q;  // total = q grid + rem
+  int rem;
+  __device__ __forceinline__ Cut(long long t, int g) : total(t), grid(g), q(t / g), rem((int)(t % g)) {}
+  __device__ __forceinline__ long long first(int c) const { return q * c + rem * c / grid; }
+  __device__ __forceinline__ int cta_of(long long tile) const {
+    int c = min(grid - 1, (int)((float)tile * (float)grid / (float)total));
+    while (first(c) > tile) --c;
+    while (first(c + 1) <= tile) ++c;
+    return c;
+  }
+};
 
 // A place on the line: tile `off` of unit (e, h); j counts the tiles of this CTA
 // in this phase (prefix units, own units), [j0, j1) is its run in the unit.
@@ -125,6 +142,12 @@ struct Cursor {
       }
       run();
     }
+  }
+  // to the first tile of the next run
+  __device__ __forceinline__ void skip_run(const Plan& p) {
+    off += j1 - j - 1;
+    j = j1 - 1;
+    next(p);
   }
   __device__ __forceinline__ bool whole() const { return first == 0 && j1 - j0 == n; }
   // the tile's part of the keys: in the prefix or not, first key, keys that are there
@@ -185,7 +208,7 @@ struct Smem {
   static constexpr int kQ = 0;  // two query tiles
   static constexpr int kRing = 2 * kTileBytes;
   static constexpr int kBars = kRing + kStages * kTileBytes;
-  static constexpr int kBytes = kBars + 1024;
+  static constexpr int kBytes = kBars + kBarBytes;
 };
 
 struct Bars {
@@ -194,8 +217,9 @@ struct Bars {
   uint32_t tmem;
   int own_e, own_h, own_off;
   long long scan[kThreads / 32];
+  long long q_at[2 * kTile];  // byte offset of a run's query rows
 };
-static_assert(sizeof(Bars) <= 1024, "barriers and scan scratch");
+static_assert(sizeof(Bars) <= kBarBytes, "barriers and scratch");
 
 struct Part {  // this CTA's part of the line
   long long start, pre_first;
@@ -253,46 +277,39 @@ __device__ __forceinline__ bool load_tiles(const Plan& p, const CUtensorMap* kma
 }
 
 // ---- query rows: gathered into the MMA's swizzled layout ----
+// 16 lanes copy a row's 16-byte chunks (fewer than 16 below head_dim 128), four
+// rows a step; where the rows start is worked out once per run.
 template <int DP, bool Pre>
 __device__ __forceinline__ bool load_queries(const Plan& p, char* smem, Bars* bars, Cursor<Pre> cur,
                                              bool wide, int& slot) {
   using S = Smem<DP>;
   const int tid = threadIdx.x - 64;  // 64 threads
-  const int chunks = (int)p.a.head_dim / 8;
-  const uint4* q = static_cast<const uint4*>(p.a.q);
+  const int c = tid & 15, r0 = tid >> 4;
+  const bool on = c < (int)p.a.head_dim / 8;
+  const char* q = static_cast<const char*>(p.a.q) + c * 16;
+  const uint32_t to = smem_u32(smem) + S::kQ + (c >> 3) * (kTile * 128);
   while (cur.live()) {
     const int rows = unit_rows<Pre>(p, cur.e);
+    named_sync(1, 64);  // the table's readers are done
+    for (int r = tid; r < rows; r += 64) {
+      const RowAt at = row_at<Pre>(p, cur.e, cur.h, r);
+      bars->q_at[r] = 2 * (at.b * p.a.q_b + at.t * p.a.q_t + at.head * p.a.q_h);
+    }
+    named_sync(1, 64);
     for (int s = 0; s < (wide ? 2 : 1); ++s, ++slot) {
       const int buf = slot & 1;
       if (slot >= 2) SY_WAIT(&bars->q_empty[buf], (slot / 2 - 1) & 1);
-      char* dst = smem + S::kQ + buf * S::kTileBytes;
-      const int count = min(kTile, rows - s * kTile) * chunks;
-      for (int i0 = tid; i0 < count; i0 += 64 * 8) {
-        uint4 x[8];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const int i = i0 + u * 64;
-          if (i < count) {
-            const RowAt at = row_at<Pre>(p, cur.e, cur.h, s * kTile + i / chunks);
-            x[u] = __ldg(q + (at.b * p.a.q_b + at.t * p.a.q_t + at.head * p.a.q_h) / 8 + i % chunks);
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const int i = i0 + u * 64;
-          if (i < count) {
-            const int r = i / chunks, c = i % chunks;
-            *reinterpret_cast<uint4*>(dst + (c >> 3) * (kTile * 128) + r * 128 +
-                                      (((c & 7) ^ (r & 7)) << 4)) = x[u];
-          }
-        }
-      }
+      const int count = min(kTile, rows - s * kTile);
+      if (on)
+        for (int r = r0; r < count; r += 4)
+          cp_async16(to + buf * S::kTileBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4),
+                     q + bars->q_at[s * kTile + r]);
+      cp_async_wait_all();
       fence_proxy_async();
       __syncwarp();
       if ((threadIdx.x & 31) == 0) mbar_arrive(&bars->q_full[buf]);
     }
-    do cur.next(p);
-    while (cur.live() && cur.j != cur.j0);
+    cur.skip_run(p);
   }
   return true;
 }
@@ -632,8 +649,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int heads = (int)p.a.kv_heads;
   total = total * heads + p.pre_total;
   Part part;
-  part.start = total * blockIdx.x / p.grid;
-  const long long stop = total * (blockIdx.x + 1) / p.grid;
+  const Cut cut(total, p.grid);
+  part.start = cut.first(blockIdx.x);
+  const long long stop = cut.first(blockIdx.x + 1);
   const long long pre_stop = min(stop, p.pre_total);
   part.pre_first = part.start;
   part.pre_count = (int)max(0ll, pre_stop - part.start);
@@ -702,17 +720,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 // ---------------------------------------------------------------------------
 // joining the parts of a row
 // ---------------------------------------------------------------------------
-// The runs of one unit, as (slot, run) pairs in line order.
 struct Runs {
   long long start, stop, phase;  // tiles of the unit, first tile of its phase
-  long long total;
-  int grid;
-  __device__ __forceinline__ int cta_of(long long tile) const {
-    return (int)(((tile + 1) * grid - 1) / total);
-  }
 };
 
-constexpr int kJoinWarps = 4, kJoinRows = 32;
+constexpr int kJoinWarps = 8, kJoinRows = 16;
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const Plan p) {
@@ -728,8 +740,9 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const Plan p) {
   const long long n = (p.starts[e + 1] - p.starts[e]) / heads;
   Runs own;
   own.start = p.pre_total + p.starts[e] + h * n, own.stop = own.start + n;
-  own.phase = p.pre_total, own.total = total, own.grid = p.grid;
-  const int c0 = n ? own.cta_of(own.start) : 0, c1 = n ? own.cta_of(own.stop - 1) : -1;
+  own.phase = p.pre_total;
+  const Cut cut(total, p.grid);
+  const int c0 = n ? cut.cta_of(own.start) : 0, c1 = n ? cut.cta_of(own.stop - 1) : -1;
   if (!p.share && n && c0 == c1 && (p.own_wide || n == 1)) return;  // already written
   const int rows = unit_rows<false>(p, e);
   const float ln2 = 0.69314718055994531f;
@@ -746,7 +759,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const Plan p) {
       pu_e = row / (2 * kTile), pu_r = row % (2 * kTile);
       pre.start = ((long long)h * p.pre_row_tiles + pu_e) * p.pre_tiles;
       pre.stop = pre.start + p.pre_tiles, pre.phase = 0;
-      pc0 = pre.cta_of(pre.start), pc1 = pre.cta_of(pre.stop - 1);
+      pc0 = cut.cta_of(pre.start), pc1 = cut.cta_of(pre.stop - 1);
     }
     const int n_pre = 2 * (pc1 - pc0 + 1), n_all = n_pre + 2 * (c1 - c0 + 1);
     for (int base = 0; base < n_all; base += 32) {
@@ -759,7 +772,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const Plan p) {
         const int cta = (is_pre ? pc0 : c0) + (k >> 1), s = k & 1;
         const Runs& u = is_pre ? pre : own;
         const bool wide = is_pre ? p.pre_wide : p.own_wide;
-        const long long c_start = total * cta / p.grid, c_stop = total * (cta + 1) / p.grid;
+        const long long c_start = cut.first(cta), c_stop = cut.first(cta + 1);
         const long long from = max(u.start, c_start), to = min(u.stop, c_stop);
         const int ur = is_pre ? pu_r : r;
         bool there = to > from;

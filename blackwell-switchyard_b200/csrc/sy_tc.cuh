@@ -152,6 +152,14 @@ __device__ __forceinline__ uint64_t policy_evict_normal() {
   return p;
 }
 
+// 16 bytes from global to shared memory by a thread, without registers
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() {
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
 // 2^x, subnormal results flushed to zero
 __device__ __forceinline__ float ex2(float x) {
   float y;
