@@ -39,6 +39,10 @@ namespace {
 
 constexpr int kTile = 128;     // keys of a tile, rows of a stream
 constexpr int kThreads = 384;  // load, MMA, 2 query warps, 2 x 4 softmax warps
+// Registers a thread: at launch (what the bound of 384 threads leaves), then per role. The shares
+// may not sum above the launch's total, or the increase would wait for ever.
+constexpr int kRegsLaunch = 168, kRegsOther = 104, kRegsSoftmax = 200;
+static_assert(128 * kRegsOther + 256 * kRegsSoftmax <= kThreads * kRegsLaunch, "register shares");
 constexpr int kBarBytes = 3072;  // barriers and scratch behind the tiles
 constexpr float kGrow = 8.f;   // log2 of the growth of a maximum that is let pass
 
@@ -469,22 +473,22 @@ __device__ __forceinline__ bool softmax_tiles(const Plan& p, Bars* bars, uint32_
     ++st.s_count;
     tc_fence_after();
     if (warp * 32 < rows) {
-      // The row is read twice, 32 columns at a time: held whole it would take
-      // every register of the thread.
-      uint32_t xa[32], xb[32];
-      tmem_ld32(s_at, xa);
+      uint32_t x[4][32];
+      tmem_ld32(s_at, x[0]);
+      tmem_ld32(s_at + 32, x[1]);
       const int keys = cur.keys(p);
       const int upto = cur.in_prefix(p) ? keys : min(keys, see - cur.key0(p));
       const bool masked = __any_sync(kFull, upto < kTile);
-      float top = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t* x = i & 1 ? xb : xa;
-        tmem_wait_ld(x);
-        if (i < 3) tmem_ld32(s_at + 32 * (i + 1), i & 1 ? xa : xb);
-        if (masked) mask_columns(x, upto - 32 * i);
-        top = fmaxf(top, row_max(x));
-      }
+      tmem_wait_ld(x[0]);
+      tmem_landed(x[1]);
+      tmem_ld32(s_at + 64, x[2]);
+      tmem_ld32(s_at + 96, x[3]);
+      if (masked) mask_columns(x[0], upto), mask_columns(x[1], upto - 32);
+      float top = fmaxf(row_max(x[0]), row_max(x[1]));
+      tmem_wait_ld(x[2]);
+      tmem_landed(x[3]);
+      if (masked) mask_columns(x[2], upto - 64), mask_columns(x[3], upto - 96);
+      top = fmaxf(top, fmaxf(row_max(x[2]), row_max(x[3])));
       // The first maximum is taken as it is; later ones only past 2^kGrow.
       const bool moves = m == -INFINITY ? top > -INFINITY : (top - m) * c > kGrow;
       if (__any_sync(kFull, moves)) {
@@ -507,28 +511,22 @@ __device__ __forceinline__ bool softmax_tiles(const Plan& p, Bars* bars, uint32_
       const float off = (m == -INFINITY ? 0.f : -m * c) + weight_shift<T>();
       const float2 c2 = make_float2(c, c), off2 = make_float2(off, off);
       float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
-      tmem_ld32(s_at, xa);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        uint32_t* x = i & 1 ? xb : xa;
-        tmem_wait_ld(x);
-        if (i < 3) tmem_ld32(s_at + 32 * (i + 1), i & 1 ? xa : xb);
-        if (masked) mask_columns(x, upto - 32 * i);
 #pragma unroll
         for (int k = 0; k < 32; k += 4) {
-          float2 u = make_float2(__uint_as_float(x[k]), __uint_as_float(x[k + 1]));
-          float2 w = make_float2(__uint_as_float(x[k + 2]), __uint_as_float(x[k + 3]));
+          float2 u = make_float2(__uint_as_float(x[i][k]), __uint_as_float(x[i][k + 1]));
+          float2 w = make_float2(__uint_as_float(x[i][k + 2]), __uint_as_float(x[i][k + 3]));
           u = __ffma2_rn(u, c2, off2);
           w = __ffma2_rn(w, c2, off2);
           u = make_float2(ex2(u.x), ex2(u.y));
           w = make_float2(ex2(w.x), ex2(w.y));
           sum0 = __fadd2_rn(sum0, u);
           sum1 = __fadd2_rn(sum1, w);
-          x[k / 2] = pack16<T>(u.x, u.y);
-          x[k / 2 + 1] = pack16<T>(w.x, w.y);
+          x[i][k / 2] = pack16<T>(u.x, u.y);
+          x[i][k / 2 + 1] = pack16<T>(w.x, w.y);
         }
-        // P takes half of S's columns: these 16 were read in this step or before
-        tmem_st16(s_at + 16 * i, x);
+        tmem_st16(s_at + 16 * i, x[i]);  // P takes half of S's columns
       }
       l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
       tmem_wait_st();
@@ -691,22 +689,27 @@ __global__ void __launch_bounds__(kThreads, 1)
               part.own_count ? bars->own_off : 0, part.own_count);
   }
   const bool pre_wide = p.pre_wide, own_wide = p.own_wide;
-  if (warp == 0) {
-    int pos = 0;
-    load_tiles<DP, true>(p, &kmap, &vmap, smem, bars, pre, pos) &&
-        load_tiles<DP, false>(p, &kmap, &vmap, smem, bars, own, pos);
-    // every copy has landed before the CTA may end
-    for (int i = max(0, pos - S::kStages); i < pos; ++i)
-      mbar_wait(&bars->full[i % S::kStages], (i / S::kStages) & 1);
-  } else if (warp == 1) {
-    MmaState st;
-    issue_mmas<DP, kBf16, true>(p, smem, bars, tmem, pre, pre_wide, st) &&
-        issue_mmas<DP, kBf16, false>(p, smem, bars, tmem, own, own_wide, st);
-  } else if (warp < 4) {
-    int slot = 0;
-    load_queries<DP, true>(p, smem, bars, pre, pre_wide, slot) &&
-        load_queries<DP, false>(p, smem, bars, own, own_wide, slot);
+  // A softmax thread holds a row of 128 scores: the other warps hand registers over.
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+    if (warp == 0) {
+      int pos = 0;
+      load_tiles<DP, true>(p, &kmap, &vmap, smem, bars, pre, pos) &&
+          load_tiles<DP, false>(p, &kmap, &vmap, smem, bars, own, pos);
+      // every copy has landed before the CTA may end
+      for (int i = max(0, pos - S::kStages); i < pos; ++i)
+        mbar_wait(&bars->full[i % S::kStages], (i / S::kStages) & 1);
+    } else if (warp == 1) {
+      MmaState st;
+      issue_mmas<DP, kBf16, true>(p, smem, bars, tmem, pre, pre_wide, st) &&
+          issue_mmas<DP, kBf16, false>(p, smem, bars, tmem, own, own_wide, st);
+    } else {
+      int slot = 0;
+      load_queries<DP, true>(p, smem, bars, pre, pre_wide, slot) &&
+          load_queries<DP, false>(p, smem, bars, own, own_wide, slot);
+    }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
     SoftState st;
     const int s = warp >= 8;
     softmax_tiles<T, DP, true>(p, bars, tmem, s, pre, pre_wide, part, st) &&
@@ -724,10 +727,10 @@ struct Runs {
   long long start, stop, phase;  // tiles of the unit, first tile of its phase
 };
 
-constexpr int kJoinWarps = 8, kJoinRows = 16;
+constexpr int kJoinWarps = 8, kJoinRows = 16, kJoinBlocks = 5;  // blocks an SM
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const Plan p) {
+__global__ void __launch_bounds__(32 * kJoinWarps, kJoinBlocks) join_kernel(const Plan p) {
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int unit_max = p.own_wide ? min(p.rows, 2 * kTile) : p.rows;
@@ -799,7 +802,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const Plan p) {
       const float* src = (is_pre ? p.pre_o : p.own_o) + at_row * DP;
       unsigned live = __ballot_sync(kFull, w > 0.f);
       while (live) {
-        constexpr int kAtOnce = 8;
+        constexpr int kAtOnce = 4;
         float4 x[kAtOnce];
         float f[kAtOnce];
         unsigned rest = live;
@@ -926,6 +929,12 @@ bool cache_map(CUtensorMap* map, const void* base, const sy_attend_args& a, int6
 
 template <typename T, int DP>
 cudaError_t launch_type(const Plan& p, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st) {
+  static const cudaError_t fits = [] {  // the register shares count on the launch's total
+    cudaFuncAttributes f;
+    const cudaError_t e = cudaFuncGetAttributes(&f, attend_kernel<T, DP>);
+    return e != cudaSuccess ? e : f.numRegs == kRegsLaunch ? cudaSuccess : cudaErrorInvalidConfiguration;
+  }();
+  if (fits != cudaSuccess) return fits;
   cudaError_t e = launch_smem(attend_kernel<T, DP>, dim3(p.grid), kThreads, Smem<DP>::kBytes, st, p,
                               k, v);
   if (e != cudaSuccess) return e;
@@ -936,6 +945,13 @@ cudaError_t launch_type(const Plan& p, const CUtensorMap& k, const CUtensorMap& 
 }
 
 }  // namespace
+
+cudaError_t take_attend_error(unsigned int* word) {
+  const cudaError_t e = cudaMemcpyFromSymbol(word, g_device_error, sizeof(*word));
+  if (e != cudaSuccess) return e;
+  const unsigned int zero = 0;
+  return cudaMemcpyToSymbol(g_device_error, &zero, sizeof(zero));
+}
 
 int64_t attend_workspace(const sy_attend_args& a, const ServingDev& dev) {
   Plan p;

@@ -81,6 +81,12 @@ __device__ __forceinline__ void tmem_wait_ld(uint32_t* r) {
                :
                : "memory");
 }
+// Further registers that the wait before has covered.
+__device__ __forceinline__ void tmem_landed(uint32_t* r) {
+  asm volatile(""
+               : SY_IO4(r, 0), SY_IO4(r, 4), SY_IO4(r, 8), SY_IO4(r, 12), SY_IO4(r, 16),
+                 SY_IO4(r, 20), SY_IO4(r, 24), SY_IO4(r, 28));
+}
 __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
