@@ -39,10 +39,6 @@ namespace {
 
 constexpr int kTile = 128;     // keys of a tile, rows of a stream
 constexpr int kThreads = 384;  // load, MMA, 2 query warps, 2 x 4 softmax warps
-// Registers a thread: at launch (what the bound of 384 threads leaves), then per role. The shares
-// may not sum above the launch's total, or the increase would wait for ever.
-constexpr int kRegsLaunch = 168, kRegsOther = 104, kRegsSoftmax = 200;
-static_assert(128 * kRegsOther + 256 * kRegsSoftmax <= kThreads * kRegsLaunch, "register shares");
 constexpr int kBarBytes = 3072;  // barriers and scratch behind the tiles
 constexpr float kGrow = 8.f;   // log2 of the growth of a maximum that is let pass
 
@@ -100,14 +96,22 @@ struct Cut {
   }
 };
 
-// A place on the line: tile `off` of unit (e, h); j counts the tiles of this CTA
-// in this phase (prefix units, own units), [j0, j1) is its run in the unit.
-template <bool Pre>
+// A CTA's part of the line: its first tile of the prefix units, and of the own
+// units the entry, head and tile it begins at.
+struct Part {
+  int pre_first, pre_count, own_e, own_h, own_off, own_count;
+};
+
+// A place on the line: tile `off` of unit (e, h) of a phase (prefix units, own
+// units); j counts the tiles of this CTA in the phase, [j0, j1) is its run in
+// the unit.
 struct Cursor {
+  bool pre;
   int e, h, n, lim, len, off, first, j, j0, j1, end;
   __device__ __forceinline__ void enter(const Plan& p) {
-    if (Pre) {
+    if (pre) {
       n = p.pre_tiles;
+      lim = len = 0;
     } else {
       len = own_len(p, e / p.own_row_tiles);
       lim = entry_limit(p, e % p.own_row_tiles, len);
@@ -119,56 +123,57 @@ struct Cursor {
     j0 = j;
     j1 = min(end, j + n - off);
   }
-  __device__ __forceinline__ void start(const Plan& p, int entry, int head, int tile, int count) {
-    e = entry, h = head, off = tile, j = 0, end = count;
-    if (count > 0) {
-      enter(p);
-      run();
+  __device__ __forceinline__ void start(const Plan& p, const Part& part, bool prefix) {
+    pre = prefix;
+    j = 0;
+    if (pre) {
+      end = part.pre_count;
+      if (end == 0) return;
+      const int unit = part.pre_first / p.pre_tiles;
+      off = part.pre_first % p.pre_tiles;
+      e = unit % p.pre_row_tiles, h = unit / p.pre_row_tiles;
+    } else {
+      end = part.own_count;
+      if (end == 0) return;
+      e = part.own_e, h = part.own_h, off = part.own_off;
     }
+    enter(p);
+    run();
   }
   __device__ __forceinline__ bool live() const { return j < end; }
-  __device__ __forceinline__ void next(const Plan& p) {
-    ++j;
-    ++off;
-    if (j < end && off == n) {
-      off = 0;
-      // prefix units are ordered (head, row tile), own units (entry, head)
-      if (Pre) {
-        if (++e == p.pre_row_tiles) e = 0, ++h;
-      } else {
-        do {
-          if (++h == (int)p.a.kv_heads) {
-            h = 0;
-            ++e;
-            enter(p);
-          }
-        } while (n == 0);
-      }
-      run();
-    }
-  }
   // to the first tile of the next run
-  __device__ __forceinline__ void skip_run(const Plan& p) {
-    off += j1 - j - 1;
-    j = j1 - 1;
-    next(p);
+  __device__ __forceinline__ void next_run(const Plan& p) {
+    j = j1;
+    if (j >= end) return;
+    off = 0;
+    // prefix units are ordered (head, row tile), own units (entry, head)
+    if (pre) {
+      if (++e == p.pre_row_tiles) e = 0, ++h;
+    } else {
+      do {
+        if (++h == (int)p.a.kv_heads) {
+          h = 0;
+          ++e;
+          enter(p);
+        }
+      } while (n == 0);
+    }
+    run();
   }
   __device__ __forceinline__ bool whole() const { return first == 0 && j1 - j0 == n; }
-  // the tile's part of the keys: in the prefix or not, first key, keys that are there
-  __device__ __forceinline__ bool in_prefix(const Plan& p) const { return Pre || off < p.lead_tiles; }
-  __device__ __forceinline__ int key0(const Plan& p) const {
-    return (Pre || off < p.lead_tiles ? off : off - p.lead_tiles) * kTile;
+  // tile `t` of the unit: in the prefix or not, its first key, the keys that are there
+  __device__ __forceinline__ bool in_prefix(const Plan& p, int t) const { return pre || t < p.lead_tiles; }
+  __device__ __forceinline__ int key0(const Plan& p, int t) const {
+    return (in_prefix(p, t) ? t : t - p.lead_tiles) * kTile;
   }
-  __device__ __forceinline__ int keys(const Plan& p) const {
-    const int upto = in_prefix(p) ? (int)p.a.prefix_len : lim;
-    return min(kTile, upto - key0(p));
+  __device__ __forceinline__ int keys(const Plan& p, int t) const {
+    return min(kTile, (in_prefix(p, t) ? (int)p.a.prefix_len : lim) - key0(p, t));
   }
 };
 
-// The row of a unit: output row (sequence, query, head), query address, and how many own keys it sees.
-template <bool Pre>
-__device__ __forceinline__ int unit_rows(const Plan& p, int e) {
-  if (Pre) {
+// The rows of a unit, and one of them: sequence, query, head.
+__device__ __forceinline__ int unit_rows(const Plan& p, bool pre, int e) {
+  if (pre) {
     const long long all = p.a.batch * p.rows, at = (long long)e * 2 * kTile;
     return (int)(p.pre_wide ? min((long long)2 * kTile, all - at) : all);
   }
@@ -177,27 +182,26 @@ __device__ __forceinline__ int unit_rows(const Plan& p, int e) {
 struct RowAt {
   int b, t, head;
 };
-template <bool Pre>
-__device__ __forceinline__ RowAt row_at(const Plan& p, int e, int h, int r) {
+__device__ __forceinline__ RowAt row_at(const Plan& p, bool pre, int e, int h, int r) {
   RowAt x;
-  if (Pre) {
-    const int row = e * 2 * kTile + r;
-    x.b = row / p.rows;
-    r = row % p.rows;
+  if (pre) {
+    r += e * 2 * kTile;
+    x.b = r / p.rows;
+    r -= x.b * p.rows;
   } else {
     x.b = e / p.own_row_tiles;
-    r += e % p.own_row_tiles * 2 * kTile;
+    r += (e - x.b * p.own_row_tiles) * 2 * kTile;
   }
   x.t = r / p.group;
-  x.head = h * p.group + r % p.group;
+  x.head = h * p.group + r - x.t * p.group;
   return x;
 }
 
 // Slot of a partial result. Own units that are wide keep only the runs that a
 // CTA shares with another: its first and its last.
-template <bool Pre>
-__device__ __forceinline__ long long slot_of(const Plan& p, int e, int h, int cta, bool began_before) {
-  if (Pre) return (long long)h * p.pre_row_tiles + e + cta;
+__device__ __forceinline__ long long slot_of(const Plan& p, bool pre, int e, int h, int cta,
+                                             bool began_before) {
+  if (pre) return (long long)h * p.pre_row_tiles + e + cta;
   if (p.own_wide) return 2ll * cta + (began_before ? 0 : 1);
   return (long long)e * p.a.kv_heads + h + cta;
 }
@@ -219,198 +223,230 @@ struct Bars {
   uint64_t full[10], empty[10];
   uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2];
   uint32_t tmem;
+  int run_tiles[2];  // tiles of the run that a query tile belongs to
+  int stop;          // a query warp gave up
   int own_e, own_h, own_off;
   long long scan[kThreads / 32];
   long long q_at[2 * kTile];  // byte offset of a run's query rows
 };
 static_assert(sizeof(Bars) <= kBarBytes, "barriers and scratch");
 
-struct Part {  // this CTA's part of the line
-  long long start, pre_first;
-  int pre_count, own_count;
-};
-
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
-  return __all_sync(kFull, mbar_wait(bar, parity));
-}
-#define SY_WAIT(bar, parity) \
-  if (!warp_wait(bar, parity)) return false
-
-// ---- loads ----
-template <int DP, bool Pre>
-__device__ __forceinline__ bool load_tiles(const Plan& p, const CUtensorMap* kmap,
-                                           const CUtensorMap* vmap, char* smem, Bars* bars,
-                                           Cursor<Pre> cur, int& pos) {
-  using S = Smem<DP>;
-  const int lane = threadIdx.x & 31;
-  const int pieces = kTile / p.box;  // boxes of a tile, per 64 columns
-  // own keys of narrow units are read once; everything else by several row tiles
-  const uint64_t policy = Pre || p.own_wide ? policy_evict_normal() : policy_evict_first();
-  for (; cur.live(); cur.next(p)) {
-    const bool pre = cur.in_prefix(p);
-    const int key0 = cur.key0(p), keys = cur.keys(p);
-    const int used = (keys + p.box - 1) / p.box;
-    const int b = Pre ? 0 : cur.e / p.own_row_tiles;
-    const int* table = pre ? p.a.prefix_pages : p.a.page_table + b * p.a.table_row;
-    const int piece = lane % pieces;
-    int page = 0, row = 0;
-    if (piece < used) {
-      const int key = key0 + piece * p.box, ps = (int)p.a.page_size;
-      page = __ldg(table + key / ps);
-      row = key % ps;
-      if (page < 0 || page >= p.a.pages) {
-        record_device_error(kDevErrBadIndex);
-        page = (int)p.a.pages;  // past the tensor: the copy fills zeros
-      }
-    }
-#pragma unroll
-    for (int kv = 0; kv < 2; ++kv, ++pos) {
-      const int stage = pos % S::kStages;
-      if (pos >= S::kStages) SY_WAIT(&bars->empty[stage], (pos / S::kStages - 1) & 1);
-      if (lane == 0)
-        mbar_arrive_expect_tx(&bars->full[stage], (uint32_t)used * p.box * 128u * (DP / 64));
-      __syncwarp();
-      char* dst = smem + S::kRing + stage * S::kTileBytes;
-      for (int i = lane; i < pieces * (DP / 64); i += 32)
-        if (piece < used)
-          tma_load_4d(dst + (i / pieces) * (kTile * 128) + piece * p.box * 128, kv ? vmap : kmap,
-                      &bars->full[stage], (i / pieces) * 64, row, cur.h, page, policy);
+// Waits are bounded; the slow way is kept out of line, as the kernel's speed
+// hangs on its code staying small (see attend_kernel).
+__device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity) {
+  const unsigned long long t0 = globaltimer_ns();
+  for (uint32_t it = 1;; ++it) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((it & 255u) == 0 && globaltimer_ns() - t0 > kWaitLimitNs) {
+      record_device_error(kDevErrWaitTimeout);
+      return false;
     }
   }
-  return true;
+}
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
+  const uint32_t b = smem_u32(bar);
+  return mbar_try_wait(b, parity) || mbar_try_wait(b, parity) || wait_long(b, parity);
+}
+// all lanes go on, or none: what follows is executed by whole warps
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+  return __all_sync(kFull, wait(bar, parity));
+}
+
+// ---- loads ----
+template <int DP>
+__device__ __forceinline__ void load_tiles(const Plan& p, const CUtensorMap* kmap,
+                                           const CUtensorMap* vmap, char* smem, Bars* bars,
+                                           const Part& part) {
+  using S = Smem<DP>;
+  const int lane = threadIdx.x & 31;
+  const int pieces = kTile / p.box;  // boxes of a tile, per 64 columns; 16 at most
+  const int piece = lane % pieces, half = lane / pieces;
+  const int ps = (int)p.a.page_size;
+  // own keys of narrow units are read once; everything else by several row tiles
+  const uint64_t once = policy_evict_first(), more = policy_evict_normal();
+  int stage = 0, filled = 0;
+  uint32_t phase = 1;  // of the buffer's release: the first round waits for nothing
+  bool ok = true;
+#pragma unroll 1
+  for (int ph = 0; ph < 2; ++ph) {
+    Cursor cur;
+    cur.start(p, part, ph == 0);
+    const uint64_t policy = ph == 0 || p.own_wide ? more : once;
+#pragma unroll 1
+    for (; ok && cur.live(); cur.next_run(p)) {
+      const int* own_table = p.a.page_table + (cur.pre ? 0 : cur.e / p.own_row_tiles) * p.a.table_row;
+#pragma unroll 1
+      for (int t = cur.first; ok && t < cur.first + cur.j1 - cur.j0; ++t) {
+        const int used = (cur.keys(p, t) + p.box - 1) / p.box;
+        const bool mine = piece < used && half < DP / 64;
+        int page = 0, row = 0;
+        if (mine) {
+          const int key = cur.key0(p, t) + piece * p.box, at = key / ps;
+          page = __ldg((cur.in_prefix(p, t) ? p.a.prefix_pages : own_table) + at);
+          row = key - at * ps;
+          if (page < 0 || page >= p.a.pages) {
+            record_device_error(kDevErrBadIndex);
+            page = (int)p.a.pages;  // past the tensor: the copy fills zeros
+          }
+        }
+#pragma unroll 1
+        for (int kv = 0; ok && kv < 2; ++kv) {
+          ok = warp_wait(&bars->empty[stage], phase);
+          if (ok) {
+            if (lane == 0)
+              mbar_arrive_expect_tx(&bars->full[stage], (uint32_t)used * p.box * 128u * (DP / 64));
+            __syncwarp();
+            if (mine)
+              tma_load_4d(smem + S::kRing + stage * S::kTileBytes + half * (kTile * 128) + piece * p.box * 128,
+                          kv ? vmap : kmap, &bars->full[stage], half * 64, row, cur.h, page, policy);
+            if (filled < S::kStages) ++filled;
+            if (++stage == S::kStages) stage = 0, phase ^= 1;
+          }
+        }
+      }
+    }
+  }
+  // every copy has landed before the CTA may end: the last round of fills
+#pragma unroll 1
+  for (int i = 0; i < filled; ++i) {
+    if (--stage < 0) stage = S::kStages - 1, phase ^= 1;
+    wait(&bars->full[stage], phase ^ 1);
+  }
 }
 
 // ---- query rows: gathered into the MMA's swizzled layout ----
 // 16 lanes copy a row's 16-byte chunks (fewer than 16 below head_dim 128), four
 // rows a step; where the rows start is worked out once per run.
-template <int DP, bool Pre>
-__device__ __forceinline__ bool load_queries(const Plan& p, char* smem, Bars* bars, Cursor<Pre> cur,
-                                             bool wide, int& slot) {
+template <int DP>
+__device__ __forceinline__ void load_queries(const Plan& p, char* smem, Bars* bars, const Part& part) {
   using S = Smem<DP>;
   const int tid = threadIdx.x - 64;  // 64 threads
   const int c = tid & 15, r0 = tid >> 4;
   const bool on = c < (int)p.a.head_dim / 8;
   const char* q = static_cast<const char*>(p.a.q) + c * 16;
   const uint32_t to = smem_u32(smem) + S::kQ + (c >> 3) * (kTile * 128);
-  while (cur.live()) {
-    const int rows = unit_rows<Pre>(p, cur.e);
-    named_sync(1, 64);  // the table's readers are done
-    for (int r = tid; r < rows; r += 64) {
-      const RowAt at = row_at<Pre>(p, cur.e, cur.h, r);
-      bars->q_at[r] = 2 * (at.b * p.a.q_b + at.t * p.a.q_t + at.head * p.a.q_h);
+  int slot = 0;
+#pragma unroll 1
+  for (int ph = 0; ph < 2; ++ph) {
+    Cursor cur;
+    cur.start(p, part, ph == 0);
+    const bool wide = ph == 0 ? p.pre_wide : p.own_wide;
+#pragma unroll 1
+    for (; cur.live(); cur.next_run(p)) {
+      const int rows = unit_rows(p, cur.pre, cur.e);
+      named_sync(1, 64);  // the table's readers are done
+#pragma unroll 1
+      for (int r = tid; r < rows; r += 64) {
+        const RowAt at = row_at(p, cur.pre, cur.e, cur.h, r);
+        bars->q_at[r] = 2 * (at.b * p.a.q_b + at.t * p.a.q_t + at.head * p.a.q_h);
+      }
+      named_sync(1, 64);
+#pragma unroll 1
+      for (int s = 0; s < (wide ? 2 : 1); ++s, ++slot) {
+        const int buf = slot & 1;
+        if (!warp_wait(&bars->q_empty[buf], ((slot >> 1) & 1) ^ 1)) {
+          bars->stop = 1;  // the other warp must not wait at the barrier alone
+        }
+        const int count = min(kTile, rows - s * kTile);
+        if (on)
+#pragma unroll 4
+          for (int r = r0; r < count; r += 4)
+            cp_async16(to + buf * S::kTileBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4),
+                       q + bars->q_at[s * kTile + r]);
+        cp_async_wait_all();
+        fence_proxy_async();
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) {
+          bars->run_tiles[buf] = cur.j1 - cur.j0;
+          mbar_arrive(&bars->q_full[buf]);
+        }
+      }
+      named_sync(1, 64);
+      if (bars->stop) return;
     }
-    named_sync(1, 64);
-    for (int s = 0; s < (wide ? 2 : 1); ++s, ++slot) {
-      const int buf = slot & 1;
-      if (slot >= 2) SY_WAIT(&bars->q_empty[buf], (slot / 2 - 1) & 1);
-      const int count = min(kTile, rows - s * kTile);
-      if (on)
-        for (int r = r0; r < count; r += 4)
-          cp_async16(to + buf * S::kTileBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4),
-                     q + bars->q_at[s * kTile + r]);
-      cp_async_wait_all();
-      fence_proxy_async();
-      __syncwarp();
-      if ((threadIdx.x & 31) == 0) mbar_arrive(&bars->q_full[buf]);
-    }
-    cur.skip_run(p);
   }
-  return true;
 }
 
 // ---- MMAs ----
+// One thread. It follows the tiles without knowing the units: the query warps
+// publish every run's length with its query tile.
 struct MmaState {
-  int pos = 0;         // ring position of the phase's first tile
-  int slot = 0;        // query slots used by S so far
+  int k_stage = 0, v_stage = 1;  // ring buffers of the next K and V tile
+  uint32_t k_phase = 0, v_phase = 0;
+  int slot = 0;          // query tiles used up
   uint32_t p_phase = 0;  // bit s: parity of stream s's next P
 };
 
-template <int DP, bool BF16, bool Pre>
-__device__ __forceinline__ bool issue_mmas(const Plan& p, char* smem, Bars* bars, uint32_t tmem,
-                                           Cursor<Pre> cur, bool wide, MmaState& st) {
+template <int DP, bool BF16>
+__device__ __forceinline__ bool issue_mmas(uint32_t base, Bars* bars, uint32_t tmem, int count,
+                                           bool wide, MmaState& st) {
   using S = Smem<DP>;
   constexpr uint32_t kIdS = f16_idesc(BF16, kTile, kTile, false);
   constexpr uint32_t kIdO = f16_idesc(BF16, kTile, DP, true);
-  const int lane = threadIdx.x & 31;
-  const uint32_t base = smem_u32(smem);
-  Cursor<Pre> ahead = cur;
-
-  // S of stream s for the tile `ahead` stands at
-  auto scores = [&](int s) -> bool {
-    const int kpos = st.pos + 2 * ahead.j, stage = kpos % S::kStages;
-    const int slots = wide ? 2 : 1;
-    const int slot = st.slot + (wide ? s : 0), buf = slot & 1;
-    if (!wide || s == 0) SY_WAIT(&bars->full[stage], (kpos / S::kStages) & 1);
-    if (ahead.j == ahead.j0) SY_WAIT(&bars->q_full[buf], (slot / 2) & 1);
-    tc_fence_after();
-    if (lane == 0) {
-      const uint64_t a = sw128_desc(base + S::kQ + buf * S::kTileBytes, 16, 1024);
-      const uint64_t b = sw128_desc(base + S::kRing + stage * S::kTileBytes, 16, 1024);
-#pragma unroll
-      for (int k = 0; k < DP / 16; ++k) {
-        const uint64_t step = (uint64_t)((k >> 2) * (kTile * 128) + (k & 3) * 32) >> 4;
-        mma_ss(tmem + s * kTile, a + step, b + step, kIdS, k > 0);
-      }
-      tc_commit(&bars->s_full[s]);
-      if (!wide || s == 1) tc_commit(&bars->empty[stage]);
-      if (ahead.j + 1 == ahead.j1) tc_commit(&bars->q_empty[buf]);
-    }
-    __syncwarp();
-    if (!wide || s == 1) {
-      if (ahead.j + 1 == ahead.j1) st.slot += slots;
-      ahead.next(p);
-    }
-    return true;
-  };
-
-  for (int i = 0; i < (wide ? 1 : 2); ++i)
-    if (ahead.live())
-      for (int s = wide ? 0 : i; s <= (wide ? 1 : i); ++s)
-        if (!scores(s)) return false;
-
-  for (; cur.live(); cur.next(p)) {
-    const int vpos = st.pos + 2 * cur.j + 1, stage = vpos % S::kStages;
-    SY_WAIT(&bars->full[stage], (vpos / S::kStages) & 1);
-    const int keys = cur.keys(p);
-    if (keys < kTile) {
-      // what lies behind the last key in its page may be anything, and 0 * NaN is NaN
-      char* v = smem + S::kRing + stage * S::kTileBytes;
-      const int n = (kTile - keys) * 8;
-      for (int half = 0; half < DP / 64; ++half)
-        for (int i = lane; i < n; i += 32)
-          *reinterpret_cast<uint4*>(v + half * (kTile * 128) + keys * 128 + i * 16) =
-              make_uint4(0, 0, 0, 0);
-      fence_proxy_async();
-      __syncwarp();
-    }
-    const uint64_t b = sw128_desc(base + S::kRing + stage * S::kTileBytes, kTile * 128, 1024);
-    for (int s = wide ? 0 : cur.j & 1; s <= (wide ? 1 : cur.j & 1); ++s) {
-      SY_WAIT(&bars->p_full[s], (st.p_phase >> s) & 1);
-      st.p_phase ^= 1u << s;
-      tc_fence_after();
-      const int step = wide ? 1 : 2;  // tiles between two of this stream
-      if (lane == 0) {
-        const bool fresh = cur.j - cur.j0 < step;
+  const uint64_t q_desc = sw128_desc(base + S::kQ, 16, 1024);
+  const uint64_t k_desc = sw128_desc(base + S::kRing, 16, 1024);
+  const uint64_t v_desc = sw128_desc(base + S::kRing, kTile * 128, 1024);
+  const int ahead = wide ? 1 : 2;  // tiles that S runs ahead of P V, and between two of a stream
+  int at = 0, run = 0;             // place in the run of the next S tile
+  uint32_t marks = 0;              // tiles j, j + 1, ..: bit 0 first, bit 1 last of a stream's run
+  // step i issues P V of tile i - ahead and S of tile i, stream by stream
+#pragma unroll 1
+  for (int i = 0; i < count + ahead; ++i) {
+    const int j = i - ahead;
+    if (j >= 0 && !wait(&bars->full[st.v_stage], st.v_phase)) return false;
+    const uint32_t mine = marks;
+    const uint64_t v = v_desc + (uint32_t)(st.v_stage * (S::kTileBytes >> 4));
+#pragma unroll 1
+    for (int s = wide ? 0 : i & 1; s <= (wide ? 1 : i & 1); ++s) {
+      const bool done = !wide || s == 1;  // with this tile's buffers
+      if (j >= 0) {
+        if (!wait(&bars->p_full[s], (st.p_phase >> s) & 1)) return false;
+        st.p_phase ^= 1u << s;
+        tc_fence_after();
 #pragma unroll
         for (int k = 0; k < kTile / 16; ++k)
-          mma_ts(tmem + 2 * kTile + s * kTile, tmem + s * kTile + k * 8, b + (uint64_t)(k * (2048 >> 4)),
-                 kIdO, k > 0 || !fresh);
-        if (!wide || s == 1) tc_commit(&bars->empty[stage]);
-        if (cur.j1 - cur.j <= step) tc_commit(&bars->o_full[s]);
+          mma_ts(tmem + 2 * kTile + s * kTile, tmem + s * kTile + k * 8,
+                 v + (uint32_t)(k * (2048 >> 4)), kIdO, k > 0 || !(mine & 1u));
+        if (mine & 2u) tc_commit(&bars->o_full[s]);
+        if (done) tc_commit(&bars->empty[st.v_stage]);
       }
-      __syncwarp();
-      if (ahead.live() && !scores(s)) return false;
+      if (i < count) {
+        const int slot = st.slot + (wide ? s : 0), buf = slot & 1;
+        if (!wait(&bars->full[st.k_stage], st.k_phase)) return false;
+        if (at == 0) {
+          if (!wait(&bars->q_full[buf], (slot >> 1) & 1)) return false;
+          run = bars->run_tiles[buf];
+        }
+        const uint64_t a = q_desc + (uint32_t)(buf * (S::kTileBytes >> 4));
+        const uint64_t b = k_desc + (uint32_t)(st.k_stage * (S::kTileBytes >> 4));
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+          const uint32_t off = ((k >> 2) * (kTile * 128) + (k & 3) * 32) >> 4;
+          mma_ss(tmem + s * kTile, a + off, b + off, kIdS, k > 0);
+        }
+        tc_commit(&bars->s_full[s]);
+        if (at + 1 == run) tc_commit(&bars->q_empty[buf]);
+        if (done) tc_commit(&bars->empty[st.k_stage]);
+      }
+    }
+    if (j >= 0) {
+      marks >>= 2;
+      st.v_stage += 2;
+      if (st.v_stage >= S::kStages) st.v_stage -= S::kStages, st.v_phase ^= 1;
+    }
+    if (i < count) {
+      // tile i stands `ahead` places behind the next P V, which is tile j + 1
+      const int place = 2 * (j >= 0 ? ahead - 1 : i);
+      marks |= ((at < ahead ? 1u : 0u) | (run - at <= ahead ? 2u : 0u)) << place;
+      st.k_stage += 2;
+      if (st.k_stage >= S::kStages) st.k_stage -= S::kStages, st.k_phase ^= 1;
+      if (++at == run) at = 0, st.slot += wide ? 2 : 1;
     }
   }
-  st.pos += 2 * cur.end;
   return true;
 }
 
 // ---- softmax ----
-struct SoftState {
-  int s_count = 0, o_count = 0;
-};
-
 template <typename T>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi);
 template <>
@@ -428,7 +464,7 @@ __device__ __forceinline__ uint32_t pack16<__half>(float lo, float hi) {
 // below 2^-20 of the highest.
 template <typename T>
 __device__ __forceinline__ constexpr float weight_shift() {
-  return sizeof(T) == 2 && std::is_same<T, __half>::value ? 6.f : 0.f;
+  return std::is_same<T, __half>::value ? 6.f : 0.f;
 }
 
 __device__ __forceinline__ void mask_columns(uint32_t* x, int upto) {
@@ -437,162 +473,203 @@ __device__ __forceinline__ void mask_columns(uint32_t* x, int upto) {
     if (k >= upto) x[k] = 0xff800000u;  // -inf
 }
 __device__ __forceinline__ float row_max(const uint32_t* x) {
-  float a = __uint_as_float(x[0]), b = __uint_as_float(x[1]);
+  float a[4];
 #pragma unroll
-  for (int k = 2; k < 32; k += 2) {
-    a = fmaxf(a, __uint_as_float(x[k]));
-    b = fmaxf(b, __uint_as_float(x[k + 1]));
-  }
-  return fmaxf(a, b);
+  for (int k = 0; k < 4; ++k) a[k] = __uint_as_float(x[k]);
+#pragma unroll
+  for (int k = 4; k < 28; k += 8)
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      a[u] = fmaxf(fmaxf(a[u], __uint_as_float(x[k + u])), __uint_as_float(x[k + 4 + u]));
+#pragma unroll
+  for (int u = 0; u < 4; ++u) a[u] = fmaxf(a[u], __uint_as_float(x[28 + u]));
+  return fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3]));
 }
 
-template <typename T, int DP, bool Pre>
-__device__ __forceinline__ bool softmax_tiles(const Plan& p, Bars* bars, uint32_t tmem, int s,
-                                              Cursor<Pre> cur, bool wide, const Part& part,
-                                              SoftState& st) {
+// The end of a stream's run: O goes out, finished if no other run or stream has
+// keys of these rows, else in fp32 with its maximum and sum.
+template <typename T, int DP>
+__device__ __forceinline__ void put_rows(const Plan& p, const Cursor& cur, int s, bool wide, int rows,
+                                         uint32_t o_at, float m, float l) {
+  const int row = min((int)threadIdx.x & 127, rows - 1);
+  const bool mine = ((int)threadIdx.x & 127) < rows;
+  const bool final = !cur.pre && !p.share && cur.whole() && (wide || cur.n == 1);
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  char* dst;
+  if (final) {
+    const RowAt at = row_at(p, false, cur.e, cur.h, (wide ? s * kTile : 0) + row);
+    const long long out_row = (at.b * p.a.q_len + at.t) * p.a.q_heads + at.head;
+    dst = static_cast<char*>(p.a.out) + out_row * p.a.head_dim * 2;
+    if (mine && p.a.lse)
+      p.a.lse[out_row] = l > 0.f ? (m * p.c - weight_shift<T>()) * 0.69314718055994531f + logf(l)
+                                 : -INFINITY;
+  } else {
+    const long long slot = 2 * slot_of(p, cur.pre, cur.e, cur.h, blockIdx.x, cur.first > 0) + s;
+    const long long at_row = slot * (cur.pre ? p.pre_slot_rows : p.own_slot_rows) + row;
+    dst = reinterpret_cast<char*>((cur.pre ? p.pre_o : p.own_o) + at_row * DP);
+    if (mine)
+      reinterpret_cast<float2*>(cur.pre ? p.pre_ml : p.own_ml)[at_row] = make_float2(m * p.c, l);
+  }
+#pragma unroll 1
+  for (int i = 0; i < DP / 32; ++i) {
+    uint32_t o[32];
+    tmem_ld32(o_at + 32 * i, o);
+    tmem_wait_ld(o);
+    if (!mine) continue;
+    if (!final) {
+#pragma unroll
+      for (int k = 0; k < 32; k += 4)
+        *reinterpret_cast<uint4*>(dst + (32 * i + k) * 4) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 32; k += 8) {
+        uint32_t w[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const float lo = __uint_as_float(o[k + 2 * u]) * inv, hi = __uint_as_float(o[k + 2 * u + 1]) * inv;
+          w[u] = l > 0.f ? pack16<T>(lo, hi) : 0u;
+        }
+        if (32 * i + k < (int)p.a.head_dim)
+          *reinterpret_cast<uint4*>(dst + (32 * i + k) * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  }
+}
+
+template <typename T, int DP>
+__device__ __forceinline__ void softmax_rows(const Plan& p, char* smem, Bars* bars, uint32_t tmem,
+                                             int s, const Part& part) {
+  using S = Smem<DP>;
   const int row = threadIdx.x & 127, warp = row >> 5;
   const uint32_t lanes = (uint32_t)warp << 21;  // TMEM lane in bits 16..31
   const uint32_t s_at = tmem + lanes + s * kTile, o_at = tmem + lanes + (2 + s) * kTile;
   const float c = p.c;
-  float m = -INFINITY, l = 0.f;
-  int rows = 0, see = 0;
-  for (; cur.live(); cur.next(p)) {
-    if (!wide && (cur.j & 1) != s) continue;
+  uint32_t s_phase = 0, o_phase = 0;
+  int base_pos = 1;  // ring position of the phase's first V tile
+#pragma unroll 1
+  for (int ph = 0; ph < 2; ++ph) {
+    Cursor cur;
+    cur.start(p, part, ph == 0);
+    const bool wide = ph == 0 ? p.pre_wide : p.own_wide;
     const int step = wide ? 1 : 2;
-    const bool fresh = cur.j - cur.j0 < step;
-    if (fresh) {
-      m = -INFINITY;
-      l = 0.f;
-      rows = unit_rows<Pre>(p, cur.e) - (wide ? s * kTile : 0);
-      if (!Pre) {  // own keys that this row sees
-        const RowAt at = row_at<Pre>(p, cur.e, cur.h, (wide ? s * kTile : 0) + min(row, rows - 1));
-        see = cur.len - (int)p.a.q_len + at.t + 1;
-      }
-    }
-    SY_WAIT(&bars->s_full[s], st.s_count & 1);
-    ++st.s_count;
-    tc_fence_after();
-    if (warp * 32 < rows) {
-      uint32_t x[4][32];
-      tmem_ld32(s_at, x[0]);
-      tmem_ld32(s_at + 32, x[1]);
-      const int keys = cur.keys(p);
-      const int upto = cur.in_prefix(p) ? keys : min(keys, see - cur.key0(p));
-      const bool masked = __any_sync(kFull, upto < kTile);
-      tmem_wait_ld(x[0]);
-      tmem_landed(x[1]);
-      tmem_ld32(s_at + 64, x[2]);
-      tmem_ld32(s_at + 96, x[3]);
-      if (masked) mask_columns(x[0], upto), mask_columns(x[1], upto - 32);
-      float top = fmaxf(row_max(x[0]), row_max(x[1]));
-      tmem_wait_ld(x[2]);
-      tmem_landed(x[3]);
-      if (masked) mask_columns(x[2], upto - 64), mask_columns(x[3], upto - 96);
-      top = fmaxf(top, fmaxf(row_max(x[2]), row_max(x[3])));
-      // The first maximum is taken as it is; later ones only past 2^kGrow.
-      const bool moves = m == -INFINITY ? top > -INFINITY : (top - m) * c > kGrow;
-      if (__any_sync(kFull, moves)) {
-        const float keep = !moves ? 1.f : m == -INFINITY ? 0.f : ex2((m - top) * c);
-        if (moves) m = top;
-        l *= keep;
-        if (!fresh) {
-          // S of this tile follows the last P V in the MMA order, so O stands still
-#pragma unroll
-          for (int i = 0; i < DP / 32; ++i) {
-            uint32_t o[32];
-            tmem_ld32(o_at + 32 * i, o);
-            tmem_wait_ld(o);
-#pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
-            tmem_st32(o_at + 32 * i, o);
+#pragma unroll 1
+    for (; cur.live(); cur.next_run(p)) {
+      // narrow: tile j of the phase is stream j & 1's
+      const int j_first = wide ? cur.j0 : cur.j0 + ((cur.j0 ^ s) & 1);
+      if (j_first >= cur.j1) continue;
+      const int rows = unit_rows(p, cur.pre, cur.e) - (wide ? s * kTile : 0);
+      const bool active = warp * 32 < rows;
+      int see = 0;  // own keys that this row sees
+      if (!cur.pre)
+        see = cur.len - (int)p.a.q_len + 1 +
+              row_at(p, false, cur.e, cur.h, (wide ? s * kTile : 0) + max(0, min(row, rows - 1))).t;
+      float m = -INFINITY, l = 0.f;
+#pragma unroll 1
+      for (int j = j_first; j < cur.j1; j += step) {
+        const int t = cur.first + j - cur.j0;
+        const int keys = cur.keys(p, t);
+        if (!warp_wait(&bars->s_full[s], s_phase)) return;
+        s_phase ^= 1;
+        tc_fence_after();
+        if (active) {
+          const int upto = cur.in_prefix(p, t) ? keys : min(keys, see - cur.key0(p, t));
+          const bool masked = __any_sync(kFull, upto < kTile);
+          float top = -INFINITY;
+          uint32_t x[32], y[32];
+          // the row is read twice, 64 columns at a time
+#pragma unroll 1
+          for (int i = 0; i < 2; ++i) {
+            tmem_ld32(s_at + 64 * i, x);
+            tmem_ld32(s_at + 64 * i + 32, y);
+            tmem_wait_ld(x);
+            tmem_landed(y);
+            if (masked) mask_columns(x, upto - 64 * i), mask_columns(y, upto - 64 * i - 32);
+            top = fmaxf(top, fmaxf(row_max(x), row_max(y)));
           }
-        }
-      }
-      const float off = (m == -INFINITY ? 0.f : -m * c) + weight_shift<T>();
-      const float2 c2 = make_float2(c, c), off2 = make_float2(off, off);
-      float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
+          // The first maximum is taken as it is; later ones only past 2^kGrow.
+          const bool moves = m == -INFINITY ? top > -INFINITY : (top - m) * c > kGrow;
+          if (__any_sync(kFull, moves)) {
+            const float keep = !moves ? 1.f : m == -INFINITY ? 0.f : ex2((m - top) * c);
+            if (moves) m = top;
+            l *= keep;
+            if (j != j_first) {
+              // S of this tile follows the stream's last P V in the MMA order: O stands still
+#pragma unroll 1
+              for (int i = 0; i < DP / 32; ++i) {
+                tmem_ld32(o_at + 32 * i, x);
+                tmem_wait_ld(x);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int k = 0; k < 32; k += 4) {
-          float2 u = make_float2(__uint_as_float(x[i][k]), __uint_as_float(x[i][k + 1]));
-          float2 w = make_float2(__uint_as_float(x[i][k + 2]), __uint_as_float(x[i][k + 3]));
-          u = __ffma2_rn(u, c2, off2);
-          w = __ffma2_rn(w, c2, off2);
-          u = make_float2(ex2(u.x), ex2(u.y));
-          w = make_float2(ex2(w.x), ex2(w.y));
-          sum0 = __fadd2_rn(sum0, u);
-          sum1 = __fadd2_rn(sum1, w);
-          x[i][k / 2] = pack16<T>(u.x, u.y);
-          x[i][k / 2 + 1] = pack16<T>(w.x, w.y);
-        }
-        tmem_st16(s_at + 16 * i, x[i]);  // P takes half of S's columns
-      }
-      l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
-      tmem_wait_st();
-    }
-    tc_fence_before();
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) mbar_arrive(&bars->p_full[s]);
-
-    if (cur.j1 - cur.j <= step) {  // this stream's last tile of the run
-      SY_WAIT(&bars->o_full[s], st.o_count & 1);
-      ++st.o_count;
-      tc_fence_after();
-      if (warp * 32 < rows) {
-        const RowAt at = row_at<Pre>(p, cur.e, cur.h, (wide ? s * kTile : 0) + min(row, rows - 1));
-        const long long out_row = (at.b * p.a.q_len + at.t) * p.a.q_heads + at.head;
-        const bool final = !Pre && !p.share && cur.whole() && (wide || cur.n == 1);
-        const float inv = l > 0.f ? 1.f / l : 0.f;
-        const bool mine = row < rows;
-        float* po = nullptr;
-        if (!final) {
-          const bool before = cur.first > 0;
-          const long long slot = 2 * slot_of<Pre>(p, cur.e, cur.h, blockIdx.x, before) + s;
-          const long long at_row = slot * (Pre ? p.pre_slot_rows : p.own_slot_rows) + min(row, rows - 1);
-          po = (Pre ? p.pre_o : p.own_o) + at_row * DP;
-          if (mine)
-            reinterpret_cast<float2*>(Pre ? p.pre_ml : p.own_ml)[at_row] = make_float2(m * c, l);
-        } else if (mine && p.a.lse) {
-          p.a.lse[out_row] =
-              l > 0.f ? m * (c * 0.69314718055994531f) + logf(l) - weight_shift<T>() * 0.69314718055994531f
-                      : -INFINITY;
-        }
-#pragma unroll
-        for (int i = 0; i < DP / 32; ++i) {
-          uint32_t o[32];
-          tmem_ld32(o_at + 32 * i, o);
-          tmem_wait_ld(o);
-          if (!final) {
-#pragma unroll
-            for (int k = 0; k < 32; k += 4)
-              if (mine)
-                *reinterpret_cast<uint4*>(po + 32 * i + k) =
-                    make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
-          } else {
-            T* out = static_cast<T*>(p.a.out) + out_row * p.a.head_dim + 32 * i;
-#pragma unroll
-            for (int k = 0; k < 32; k += 8) {
-              uint4 w;
-              float f[8];
-#pragma unroll
-              for (int u = 0; u < 8; ++u) f[u] = l > 0.f ? __uint_as_float(o[k + u]) * inv : 0.f;
-              w = make_uint4(pack16<T>(f[0], f[1]), pack16<T>(f[2], f[3]), pack16<T>(f[4], f[5]),
-                             pack16<T>(f[6], f[7]));
-              if (mine && 32 * i + k < (int)p.a.head_dim) *reinterpret_cast<uint4*>(out + k) = w;
+                for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) * keep);
+                tmem_st32(o_at + 32 * i, x);
+              }
             }
           }
+          const float off = (m == -INFINITY ? 0.f : -m * c) + weight_shift<T>();
+          const float2 c2 = make_float2(c, c), off2 = make_float2(off, off);
+          float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
+#pragma unroll 1
+          for (int i = 0; i < 2; ++i) {
+            tmem_ld32(s_at + 64 * i, x);
+            tmem_ld32(s_at + 64 * i + 32, y);
+            tmem_wait_ld(x);
+            tmem_landed(y);
+            if (masked) mask_columns(x, upto - 64 * i), mask_columns(y, upto - 64 * i - 32);
+            uint32_t pk[32];
+#pragma unroll
+            for (int k = 0; k < 64; k += 4) {
+              const uint32_t* z = (k < 32 ? x : y) + (k & 31);
+              float2 u = make_float2(__uint_as_float(z[0]), __uint_as_float(z[1]));
+              float2 w = make_float2(__uint_as_float(z[2]), __uint_as_float(z[3]));
+              u = __ffma2_rn(u, c2, off2);
+              w = __ffma2_rn(w, c2, off2);
+              u = make_float2(ex2(u.x), ex2(u.y));
+              w = make_float2(ex2(w.x), ex2(w.y));
+              sum0 = __fadd2_rn(sum0, u);
+              sum1 = __fadd2_rn(sum1, w);
+              pk[k / 2] = pack16<T>(u.x, u.y);
+              pk[k / 2 + 1] = pack16<T>(w.x, w.y);
+            }
+            tmem_st32(s_at + 32 * i, pk);  // P takes the first half of S's columns, already read
+          }
+          l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
+          tmem_wait_st();
         }
-        tc_fence_before();  // the next run's P V overwrites O after the next p_full
+        if (keys < kTile) {
+          // What lies behind the last key in its page may be anything, and 0 * NaN
+          // is NaN: clear V there. Both streams of a wide unit do, each before its
+          // own P V.
+          const int vpos = base_pos + 2 * j, stage = vpos % S::kStages;
+          if (!warp_wait(&bars->full[stage], (vpos / S::kStages) & 1)) return;
+          char* v = smem + S::kRing + stage * S::kTileBytes + keys * 128;
+#pragma unroll 1
+          for (int i = row; i < (kTile - keys) * 8; i += 128)
+#pragma unroll
+            for (int half = 0; half < DP / 64; ++half)
+              *reinterpret_cast<uint4*>(v + half * (kTile * 128) + i * 16) = make_uint4(0, 0, 0, 0);
+          fence_proxy_async();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive(&bars->p_full[s]);
       }
+      if (!warp_wait(&bars->o_full[s], o_phase)) return;
+      o_phase ^= 1;
+      tc_fence_after();
+      if (active) put_rows<T, DP>(p, cur, s, wide, rows, o_at, m, l);
+      tc_fence_before();  // the next run's P V overwrites O after the next p_full
     }
+    base_pos += 2 * cur.end;
   }
-  return true;
 }
 
+// The kernel is latency all the way (a tile's S, softmax and P V follow one
+// another, twelve warps run different code), and instructions that come from L2
+// cost ten times those in the SM's cache: with both phases and every chunk
+// unrolled the code was 190 KB and a tile took 3 to 7 times as long. So the
+// phases share their code and the loops over chunks are real loops.
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads, 1)
-    attend_kernel(const Plan p, const __grid_constant__ CUtensorMap kmap,
+    attend_kernel(const __grid_constant__ Plan p, const __grid_constant__ CUtensorMap kmap,
                   const __grid_constant__ CUtensorMap vmap) {
   using S = Smem<DP>;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
@@ -605,15 +682,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     return;
   }
 
-  // where this CTA's part of the line starts
+  // where this CTA's part of the line starts: a scan over the entries
   const int per = (p.entries + kThreads - 1) / kThreads;
   const int e_first = min(p.entries, tid * per), e_last = min(p.entries, e_first + per);
   long long mine = 0;
+#pragma unroll 1
   for (int e = e_first; e < e_last; ++e) {
     const int b = e / p.own_row_tiles;
     const int len = own_len(p, b);
     if (blockIdx.x == 0 && len != p.a.kv_lens[b]) record_device_error(kDevErrBadIndex);
-    mine += entry_tiles(p, entry_limit(p, e % p.own_row_tiles, len));
+    mine += entry_tiles(p, entry_limit(p, e - b * p.own_row_tiles, len));
   }
   long long upto = mine;
 #pragma unroll
@@ -623,10 +701,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (lane == 31) bars->scan[warp] = upto;
   if (tid == 0) {
+#pragma unroll 1
     for (int i = 0; i < S::kStages; ++i) {
       mbar_init(&bars->full[i], 1);
       mbar_init(&bars->empty[i], 1);
     }
+#pragma unroll 1
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars->q_full[i], 2);
       mbar_init(&bars->q_empty[i], 1);
@@ -634,34 +714,37 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&bars->p_full[i], 4);
       mbar_init(&bars->o_full[i], 1);
     }
+    bars->stop = 0;
     mbar_fence_init();
     tma_prefetch_map(&kmap);
     tma_prefetch_map(&vmap);
   }
   __syncthreads();
   long long total = 0;
+#pragma unroll 1
   for (int w = 0; w < kThreads / 32; ++w) {
     if (w < warp) upto += bars->scan[w];
     total += bars->scan[w];
   }
   const int heads = (int)p.a.kv_heads;
   total = total * heads + p.pre_total;
-  Part part;
   const Cut cut(total, p.grid);
-  part.start = cut.first(blockIdx.x);
-  const long long stop = cut.first(blockIdx.x + 1);
-  const long long pre_stop = min(stop, p.pre_total);
-  part.pre_first = part.start;
-  part.pre_count = (int)max(0ll, pre_stop - part.start);
-  const long long own_first = max(part.start, p.pre_total) - p.pre_total;
-  part.own_count = (int)max(0ll, stop - p.pre_total - own_first);
+  const long long from = cut.first(blockIdx.x), to = cut.first(blockIdx.x + 1);
+  const long long own_first = max(from, p.pre_total) - p.pre_total;
+  Part part;
+  part.pre_first = (int)min(from, p.pre_total);
+  part.pre_count = (int)max(0ll, min(to, p.pre_total) - from);
+  part.own_count = (int)max(0ll, to - p.pre_total - own_first);
   long long before = (upto - mine) * heads;
+#pragma unroll 1
   for (int e = e_first; e < e_last; ++e) {
-    const int n = entry_tiles(p, entry_limit(p, e % p.own_row_tiles, own_len(p, e / p.own_row_tiles)));
-    if (own_first >= before && own_first < before + (long long)n * heads) {
+    const int b = e / p.own_row_tiles;
+    const int n = entry_tiles(p, entry_limit(p, e - b * p.own_row_tiles, own_len(p, b)));
+    const long long rel = own_first - before;
+    if (rel >= 0 && rel < (long long)n * heads) {
       bars->own_e = e;
-      bars->own_h = (int)((own_first - before) / n);
-      bars->own_off = (int)((own_first - before) % n);
+      bars->own_h = (int)rel / n;
+      bars->own_off = (int)rel % n;
     }
     if (blockIdx.x == 0) p.starts[e] = before;
     before += (long long)n * heads;
@@ -677,43 +760,24 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars->tmem;
+  part.own_e = bars->own_e, part.own_h = bars->own_h, part.own_off = bars->own_off;
 
-  Cursor<true> pre;
-  Cursor<false> own;
-  {
-    const long long unit = p.pre_tiles > 0 ? part.pre_first / p.pre_tiles : 0;
-    pre.start(p, part.pre_count ? (int)(unit % p.pre_row_tiles) : 0,
-              part.pre_count ? (int)(unit / p.pre_row_tiles) : 0,
-              part.pre_count ? (int)(part.pre_first % p.pre_tiles) : 0, part.pre_count);
-    own.start(p, part.own_count ? bars->own_e : 0, part.own_count ? bars->own_h : 0,
-              part.own_count ? bars->own_off : 0, part.own_count);
-  }
-  const bool pre_wide = p.pre_wide, own_wide = p.own_wide;
-  // A softmax thread holds a row of 128 scores: the other warps hand registers over.
-  if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
-    if (warp == 0) {
-      int pos = 0;
-      load_tiles<DP, true>(p, &kmap, &vmap, smem, bars, pre, pos) &&
-          load_tiles<DP, false>(p, &kmap, &vmap, smem, bars, own, pos);
-      // every copy has landed before the CTA may end
-      for (int i = max(0, pos - S::kStages); i < pos; ++i)
-        mbar_wait(&bars->full[i % S::kStages], (i / S::kStages) & 1);
-    } else if (warp == 1) {
+  if (warp == 0) {
+    load_tiles<DP>(p, &kmap, &vmap, smem, bars, part);
+  } else if (warp == 1) {
+    if (lane == 0) {
       MmaState st;
-      issue_mmas<DP, kBf16, true>(p, smem, bars, tmem, pre, pre_wide, st) &&
-          issue_mmas<DP, kBf16, false>(p, smem, bars, tmem, own, own_wide, st);
-    } else {
-      int slot = 0;
-      load_queries<DP, true>(p, smem, bars, pre, pre_wide, slot) &&
-          load_queries<DP, false>(p, smem, bars, own, own_wide, slot);
+      bool ok = true;
+#pragma unroll 1
+      for (int ph = 0; ok && ph < 2; ++ph)
+        ok = issue_mmas<DP, kBf16>(smem_u32(smem), bars, tmem, ph ? part.own_count : part.pre_count,
+                                   ph ? p.own_wide : p.pre_wide, st);
     }
+    __syncwarp();
+  } else if (warp < 4) {
+    load_queries<DP>(p, smem, bars, part);
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-    SoftState st;
-    const int s = warp >= 8;
-    softmax_tiles<T, DP, true>(p, bars, tmem, s, pre, pre_wide, part, st) &&
-        softmax_tiles<T, DP, false>(p, bars, tmem, s, own, own_wide, part, st);
+    softmax_rows<T, DP>(p, smem, bars, tmem, warp >= 8, part);
   }
   tc_fence_before();
   __syncthreads();
@@ -747,10 +811,10 @@ __global__ void __launch_bounds__(32 * kJoinWarps, kJoinBlocks) join_kernel(cons
   const Cut cut(total, p.grid);
   const int c0 = n ? cut.cta_of(own.start) : 0, c1 = n ? cut.cta_of(own.stop - 1) : -1;
   if (!p.share && n && c0 == c1 && (p.own_wide || n == 1)) return;  // already written
-  const int rows = unit_rows<false>(p, e);
+  const int rows = unit_rows(p, false, e);
   const float ln2 = 0.69314718055994531f;
   for (int r = r0 + warp; r < min(rows, r0 + kJoinRows); r += kJoinWarps) {
-    const RowAt at = row_at<false>(p, e, h, r);
+    const RowAt at = row_at(p, false, e, h, r);
     const long long out_row = (at.b * p.a.q_len + at.t) * p.a.q_heads + at.head;
     float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -785,8 +849,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps, kJoinBlocks) join_kernel(cons
           there = there && (to - from >= 2 || ((from - max(c_start, u.phase)) & 1) == s);
         if (there) {
           const long long slot =
-              2 * (is_pre ? slot_of<true>(p, pu_e, h, cta, false)
-                          : slot_of<false>(p, e, h, cta, u.start < c_start)) + s;
+              2 * slot_of(p, is_pre, is_pre ? pu_e : e, h, cta, u.start < c_start) + s;
           at_row = slot * (is_pre ? p.pre_slot_rows : p.own_slot_rows) + (wide ? ur & 127 : ur);
           const float2 ml = reinterpret_cast<const float2*>(is_pre ? p.pre_ml : p.own_ml)[at_row];
           if (ml.y > 0.f) cm = ml.x, cl = ml.y;
@@ -929,12 +992,6 @@ bool cache_map(CUtensorMap* map, const void* base, const sy_attend_args& a, int6
 
 template <typename T, int DP>
 cudaError_t launch_type(const Plan& p, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st) {
-  static const cudaError_t fits = [] {  // the register shares count on the launch's total
-    cudaFuncAttributes f;
-    const cudaError_t e = cudaFuncGetAttributes(&f, attend_kernel<T, DP>);
-    return e != cudaSuccess ? e : f.numRegs == kRegsLaunch ? cudaSuccess : cudaErrorInvalidConfiguration;
-  }();
-  if (fits != cudaSuccess) return fits;
   cudaError_t e = launch_smem(attend_kernel<T, DP>, dim3(p.grid), kThreads, Smem<DP>::kBytes, st, p,
                               k, v);
   if (e != cudaSuccess) return e;
