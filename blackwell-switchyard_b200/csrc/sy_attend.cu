@@ -17,6 +17,9 @@
 // needs none of them. All of this is decided by sizes; the result depends only
 // on sizes, lengths and the number of SMs.
 //
+// Every unit also stands on the line with a few places of its own for what a
+// run costs beside its tiles (query rows in, O out, the pipeline's filling).
+//
 // CTA. 12 warps: one loads K and V tiles by TMA through a ring of buffers (the
 // pages' rows land in tile order, so a page may end inside a tile), one issues
 // the MMAs, two gather query rows, and two streams of four warps each own 128
@@ -56,9 +59,10 @@ struct Plan {
   int grid;              // CTAs of the main kernel
   float c;               // scale * log2(e)
   int pre_slot_rows, own_slot_rows;
-  long long pre_total;   // tiles of all prefix units
+  int pre_extra, own_extra;  // places of a unit on the line beside its tiles
+  long long pre_total;   // places of all prefix units
   // workspace
-  long long* starts;     // [entries + 1] tiles before an entry's units
+  long long* starts;     // [entries + 1] places before an entry's units
   float *pre_ml, *pre_o, *own_ml, *own_o;
 };
 
@@ -79,8 +83,10 @@ __device__ __forceinline__ int entry_limit(const Plan& p, int row_tile, int len)
 __device__ __forceinline__ int entry_tiles(const Plan& p, int lim) {
   return p.lead_tiles + (lim + kTile - 1) / kTile;
 }
+// places of a unit of n tiles; its tiles are the last n of them
+__device__ __forceinline__ int own_places(const Plan& p, int n) { return n > 0 ? n + p.own_extra : 0; }
 
-// The line's cut: CTA c has the tiles [first(c), first(c + 1)).
+// The line's cut: CTA c has the places [first(c), first(c + 1)).
 struct Cut {
   long long total;
   int grid;
@@ -88,16 +94,16 @@ struct Cut {
   int rem;
   __device__ __forceinline__ Cut(long long t, int g) : total(t), grid(g), q(t / g), rem((int)(t % g)) {}
   __device__ __forceinline__ long long first(int c) const { return q * c + rem * c / grid; }
-  __device__ __forceinline__ int cta_of(long long tile) const {
-    int c = min(grid - 1, (int)((float)tile * (float)grid / (float)total));
-    while (first(c) > tile) --c;
-    while (first(c + 1) <= tile) ++c;
+  __device__ __forceinline__ int cta_of(long long place) const {
+    int c = min(grid - 1, (int)((float)place * (float)grid / (float)total));
+    while (first(c) > place) --c;
+    while (first(c + 1) <= place) ++c;
     return c;
   }
 };
 
-// A CTA's part of the line: its first tile of the prefix units, and of the own
-// units the entry, head and tile it begins at.
+// A CTA's part of the line in tiles: the first of the prefix units' tiles, the
+// entry, head and tile it begins at in the own units, and how many of each.
 struct Part {
   int pre_first, pre_count, own_e, own_h, own_off, own_count;
 };
@@ -225,7 +231,7 @@ struct Bars {
   uint32_t tmem;
   int run_tiles[2];  // tiles of the run that a query tile belongs to
   int stop;          // a query warp gave up
-  int own_e, own_h, own_off;
+  int own_e, own_h, own_off, own_start, own_stop;
   long long scan[kThreads / 32];
   long long q_at[2 * kTile];  // byte offset of a run's query rows
 };
@@ -486,6 +492,15 @@ __device__ __forceinline__ float row_max(const uint32_t* x) {
   return fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3]));
 }
 
+// Where a stream's partial result of a row stands.
+__device__ __forceinline__ long long part_at(const Plan& p, const Cursor& cur, int s, int row) {
+  const long long slot = 2 * slot_of(p, cur.pre, cur.e, cur.h, blockIdx.x, cur.first > 0) + s;
+  return slot * (cur.pre ? p.pre_slot_rows : p.own_slot_rows) + row;
+}
+__device__ __forceinline__ float2& part_ml(const Plan& p, const Cursor& cur, int s, int row) {
+  return reinterpret_cast<float2*>(cur.pre ? p.pre_ml : p.own_ml)[part_at(p, cur, s, row)];
+}
+
 // The end of a stream's run: O goes out, finished if no other run or stream has
 // keys of these rows, else in fp32 with its maximum and sum.
 template <typename T, int DP>
@@ -504,11 +519,8 @@ __device__ __forceinline__ void put_rows(const Plan& p, const Cursor& cur, int s
       p.a.lse[out_row] = l > 0.f ? (m * p.c - weight_shift<T>()) * 0.69314718055994531f + logf(l)
                                  : -INFINITY;
   } else {
-    const long long slot = 2 * slot_of(p, cur.pre, cur.e, cur.h, blockIdx.x, cur.first > 0) + s;
-    const long long at_row = slot * (cur.pre ? p.pre_slot_rows : p.own_slot_rows) + row;
-    dst = reinterpret_cast<char*>((cur.pre ? p.pre_o : p.own_o) + at_row * DP);
-    if (mine)
-      reinterpret_cast<float2*>(cur.pre ? p.pre_ml : p.own_ml)[at_row] = make_float2(m * p.c, l);
+    dst = reinterpret_cast<char*>((cur.pre ? p.pre_o : p.own_o) + part_at(p, cur, s, row) * DP);
+    if (mine) part_ml(p, cur, s, row) = make_float2(m * p.c, l);
   }
 #pragma unroll 1
   for (int i = 0; i < DP / 32; ++i) {
@@ -556,8 +568,11 @@ __device__ __forceinline__ void softmax_rows(const Plan& p, char* smem, Bars* ba
     for (; cur.live(); cur.next_run(p)) {
       // narrow: tile j of the phase is stream j & 1's
       const int j_first = wide ? cur.j0 : cur.j0 + ((cur.j0 ^ s) & 1);
-      if (j_first >= cur.j1) continue;
       const int rows = unit_rows(p, cur.pre, cur.e) - (wide ? s * kTile : 0);
+      if (j_first >= cur.j1) {  // a run of one tile, the other stream's
+        if (row < rows) part_ml(p, cur, s, row) = make_float2(-INFINITY, 0.f);
+        continue;
+      }
       const bool active = warp * 32 < rows;
       int see = 0;  // own keys that this row sees
       if (!cur.pre)
@@ -575,16 +590,14 @@ __device__ __forceinline__ void softmax_rows(const Plan& p, char* smem, Bars* ba
           const int upto = cur.in_prefix(p, t) ? keys : min(keys, see - cur.key0(p, t));
           const bool masked = __any_sync(kFull, upto < kTile);
           float top = -INFINITY;
-          uint32_t x[32], y[32];
-          // the row is read twice, 64 columns at a time
+          uint32_t x[32];
+          // the row is read twice, 32 columns at a time
 #pragma unroll 1
-          for (int i = 0; i < 2; ++i) {
-            tmem_ld32(s_at + 64 * i, x);
-            tmem_ld32(s_at + 64 * i + 32, y);
+          for (int i = 0; i < kTile; i += 32) {
+            tmem_ld32(s_at + i, x);
             tmem_wait_ld(x);
-            tmem_landed(y);
-            if (masked) mask_columns(x, upto - 64 * i), mask_columns(y, upto - 64 * i - 32);
-            top = fmaxf(top, fmaxf(row_max(x), row_max(y)));
+            if (masked) mask_columns(x, upto - i);
+            top = fmaxf(top, row_max(x));
           }
           // The first maximum is taken as it is; later ones only past 2^kGrow.
           const bool moves = m == -INFINITY ? top > -INFINITY : (top - m) * c > kGrow;
@@ -608,28 +621,24 @@ __device__ __forceinline__ void softmax_rows(const Plan& p, char* smem, Bars* ba
           const float2 c2 = make_float2(c, c), off2 = make_float2(off, off);
           float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
 #pragma unroll 1
-          for (int i = 0; i < 2; ++i) {
-            tmem_ld32(s_at + 64 * i, x);
-            tmem_ld32(s_at + 64 * i + 32, y);
+          for (int i = 0; i < kTile; i += 32) {
+            tmem_ld32(s_at + i, x);
             tmem_wait_ld(x);
-            tmem_landed(y);
-            if (masked) mask_columns(x, upto - 64 * i), mask_columns(y, upto - 64 * i - 32);
-            uint32_t pk[32];
+            if (masked) mask_columns(x, upto - i);
 #pragma unroll
-            for (int k = 0; k < 64; k += 4) {
-              const uint32_t* z = (k < 32 ? x : y) + (k & 31);
-              float2 u = make_float2(__uint_as_float(z[0]), __uint_as_float(z[1]));
-              float2 w = make_float2(__uint_as_float(z[2]), __uint_as_float(z[3]));
+            for (int k = 0; k < 32; k += 4) {
+              float2 u = make_float2(__uint_as_float(x[k]), __uint_as_float(x[k + 1]));
+              float2 w = make_float2(__uint_as_float(x[k + 2]), __uint_as_float(x[k + 3]));
               u = __ffma2_rn(u, c2, off2);
               w = __ffma2_rn(w, c2, off2);
               u = make_float2(ex2(u.x), ex2(u.y));
               w = make_float2(ex2(w.x), ex2(w.y));
               sum0 = __fadd2_rn(sum0, u);
               sum1 = __fadd2_rn(sum1, w);
-              pk[k / 2] = pack16<T>(u.x, u.y);
-              pk[k / 2 + 1] = pack16<T>(w.x, w.y);
+              x[k / 2] = pack16<T>(u.x, u.y);
+              x[k / 2 + 1] = pack16<T>(w.x, w.y);
             }
-            tmem_st32(s_at + 32 * i, pk);  // P takes the first half of S's columns, already read
+            tmem_st16(s_at + i / 2, x);  // P takes the first half of S's columns, already read
           }
           l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
           tmem_wait_st();
@@ -685,13 +694,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   // where this CTA's part of the line starts: a scan over the entries
   const int per = (p.entries + kThreads - 1) / kThreads;
   const int e_first = min(p.entries, tid * per), e_last = min(p.entries, e_first + per);
-  long long mine = 0;
+  long long mine = 0;  // places in the low half, tiles in the high half, both per head
 #pragma unroll 1
   for (int e = e_first; e < e_last; ++e) {
     const int b = e / p.own_row_tiles;
     const int len = own_len(p, b);
     if (blockIdx.x == 0 && len != p.a.kv_lens[b]) record_device_error(kDevErrBadIndex);
-    mine += entry_tiles(p, entry_limit(p, e - b * p.own_row_tiles, len));
+    const int n = entry_tiles(p, entry_limit(p, e - b * p.own_row_tiles, len));
+    mine += own_places(p, n) + ((long long)n << 32);
   }
   long long upto = mine;
 #pragma unroll
@@ -727,29 +737,46 @@ __global__ void __launch_bounds__(kThreads, 1)
     total += bars->scan[w];
   }
   const int heads = (int)p.a.kv_heads;
-  total = total * heads + p.pre_total;
+  total = (total & 0xffffffffll) * heads + p.pre_total;
   const Cut cut(total, p.grid);
   const long long from = cut.first(blockIdx.x), to = cut.first(blockIdx.x + 1);
-  const long long own_first = max(from, p.pre_total) - p.pre_total;
+  auto pre_tiles_before = [&](long long place) -> int {
+    if (place <= 0 || p.pre_total == 0) return 0;
+    const int len = p.pre_tiles + p.pre_extra;
+    const int at = (int)min(place, p.pre_total), unit = at / len;
+    return unit * p.pre_tiles + max(0, at - unit * len - p.pre_extra);
+  };
   Part part;
-  part.pre_first = (int)min(from, p.pre_total);
-  part.pre_count = (int)max(0ll, min(to, p.pre_total) - from);
-  part.own_count = (int)max(0ll, to - p.pre_total - own_first);
-  long long before = (upto - mine) * heads;
+  part.pre_first = pre_tiles_before(from);
+  part.pre_count = pre_tiles_before(to) - part.pre_first;
+  // The own part's ends: the thread whose entries they fall into works them out.
+  const long long own_from = max(from, p.pre_total) - p.pre_total, own_to = to - p.pre_total;
+  long long before = ((upto - mine) & 0xffffffffll) * heads, tiles = ((upto - mine) >> 32) * heads;
 #pragma unroll 1
   for (int e = e_first; e < e_last; ++e) {
     const int b = e / p.own_row_tiles;
     const int n = entry_tiles(p, entry_limit(p, e - b * p.own_row_tiles, own_len(p, b)));
-    const long long rel = own_first - before;
-    if (rel >= 0 && rel < (long long)n * heads) {
-      bars->own_e = e;
-      bars->own_h = (int)rel / n;
-      bars->own_off = (int)rel % n;
-    }
+    const int len = own_places(p, n);
     if (blockIdx.x == 0) p.starts[e] = before;
-    before += (long long)n * heads;
+#pragma unroll 1
+    for (int end = 0; end < 2; ++end) {
+      const long long rel = (end ? own_to : own_from) - before;
+      if (rel < end || rel >= (long long)len * heads + end) continue;
+      const int h = (int)(rel - end) / len, off = max(0, (int)(rel - (long long)h * len) - p.own_extra);
+      if (end) {
+        bars->own_stop = (int)(tiles + (long long)h * n + off);
+      } else {
+        bars->own_e = e, bars->own_h = h, bars->own_off = off;
+        bars->own_start = (int)(tiles + (long long)h * n + off);
+      }
+    }
+    before += (long long)len * heads;
+    tiles += (long long)n * heads;
   }
   if (blockIdx.x == 0 && tid == kThreads - 1) p.starts[p.entries] = total - p.pre_total;
+  __syncthreads();
+  part.own_e = bars->own_e, part.own_h = bars->own_h, part.own_off = bars->own_off;
+  part.own_count = own_to > own_from ? bars->own_stop - bars->own_start : 0;
   if (part.pre_count + part.own_count == 0) return;
 
   if (warp == 2) tmem_alloc(&bars->tmem, 512);
@@ -760,7 +787,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars->tmem;
-  part.own_e = bars->own_e, part.own_h = bars->own_h, part.own_off = bars->own_off;
 
   if (warp == 0) {
     load_tiles<DP>(p, &kmap, &vmap, smem, bars, part);
@@ -787,8 +813,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 // ---------------------------------------------------------------------------
 // joining the parts of a row
 // ---------------------------------------------------------------------------
-struct Runs {
-  long long start, stop, phase;  // tiles of the unit, first tile of its phase
+// The places of a unit's tiles.
+struct Places {
+  long long start, stop;
 };
 
 constexpr int kJoinWarps = 8, kJoinRows = 16, kJoinBlocks = 5;  // blocks an SM
@@ -804,10 +831,11 @@ __global__ void __launch_bounds__(32 * kJoinWarps, kJoinBlocks) join_kernel(cons
   const int e = (int)(block / groups / heads), h = (int)(block / groups % heads);
   const int r0 = (int)(block % groups) * kJoinRows;
   const long long own_total = p.starts[p.entries], total = own_total + p.pre_total;
-  const long long n = (p.starts[e + 1] - p.starts[e]) / heads;
-  Runs own;
-  own.start = p.pre_total + p.starts[e] + h * n, own.stop = own.start + n;
-  own.phase = p.pre_total;
+  const int places = (int)(p.starts[e + 1] - p.starts[e]) / heads;
+  Places own;
+  own.stop = p.pre_total + p.starts[e] + (h + 1ll) * places;
+  own.start = own.stop - places + (places ? p.own_extra : 0);
+  const int n = (int)(own.stop - own.start);
   const Cut cut(total, p.grid);
   const int c0 = n ? cut.cta_of(own.start) : 0, c1 = n ? cut.cta_of(own.stop - 1) : -1;
   if (!p.share && n && c0 == c1 && (p.own_wide || n == 1)) return;  // already written
@@ -820,12 +848,12 @@ __global__ void __launch_bounds__(32 * kJoinWarps, kJoinBlocks) join_kernel(cons
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     // candidates: (CTA, stream) of the prefix unit, then of the own unit
     int pu_e = 0, pu_r = 0, pc0 = 0, pc1 = -1;
-    Runs pre = own;
+    Places pre = own;
     if (p.share) {
       const int row = at.b * p.rows + r;
       pu_e = row / (2 * kTile), pu_r = row % (2 * kTile);
-      pre.start = ((long long)h * p.pre_row_tiles + pu_e) * p.pre_tiles;
-      pre.stop = pre.start + p.pre_tiles, pre.phase = 0;
+      pre.stop = ((long long)h * p.pre_row_tiles + pu_e + 1) * (p.pre_tiles + p.pre_extra);
+      pre.start = pre.stop - p.pre_tiles;
       pc0 = cut.cta_of(pre.start), pc1 = cut.cta_of(pre.stop - 1);
     }
     const int n_pre = 2 * (pc1 - pc0 + 1), n_all = n_pre + 2 * (c1 - c0 + 1);
@@ -837,16 +865,11 @@ __global__ void __launch_bounds__(32 * kJoinWarps, kJoinBlocks) join_kernel(cons
       if (i < n_all) {
         const int k = is_pre ? i : i - n_pre;
         const int cta = (is_pre ? pc0 : c0) + (k >> 1), s = k & 1;
-        const Runs& u = is_pre ? pre : own;
+        const Places& u = is_pre ? pre : own;
         const bool wide = is_pre ? p.pre_wide : p.own_wide;
         const long long c_start = cut.first(cta), c_stop = cut.first(cta + 1);
-        const long long from = max(u.start, c_start), to = min(u.stop, c_stop);
         const int ur = is_pre ? pu_r : r;
-        bool there = to > from;
-        if (wide)
-          there = there && (ur >> 7) == s;
-        else  // tile j of a CTA's phase went to stream j & 1
-          there = there && (to - from >= 2 || ((from - max(c_start, u.phase)) & 1) == s);
+        const bool there = min(u.stop, c_stop) > max(u.start, c_start) && (!wide || (ur >> 7) == s);
         if (there) {
           const long long slot =
               2 * slot_of(p, is_pre, is_pre ? pu_e : e, h, cta, u.start < c_start) + s;
@@ -930,7 +953,9 @@ int64_t make_plan(const sy_attend_args& a, int sms, Plan* p, char* ws) {
   p->pre_row_tiles = p->pre_wide ? (int)((pre_rows + 2 * kTile - 1) / (2 * kTile)) : 1;
   p->own_row_tiles = p->own_wide ? (p->rows + 2 * kTile - 1) / (2 * kTile) : 1;
   p->entries = (int)(a.batch * p->own_row_tiles);
-  p->pre_total = (int64_t)p->pre_tiles * p->pre_row_tiles * a.kv_heads;
+  p->pre_extra = p->pre_wide ? 2 : 1;
+  p->own_extra = p->own_wide ? 2 : 1;
+  p->pre_total = p->share ? (int64_t)(p->pre_tiles + p->pre_extra) * p->pre_row_tiles * a.kv_heads : 0;
   p->box = (int)(a.page_size & -a.page_size);
   if (p->box > kTile) p->box = kTile;
   p->grid = sms;
