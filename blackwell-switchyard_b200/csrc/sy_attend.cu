@@ -59,7 +59,8 @@ struct Plan {
   int grid;              // CTAs of the main kernel
   float c;               // scale * log2(e)
   int pre_slot_rows, own_slot_rows;
-  int pre_extra, own_extra;  // places of a unit on the line beside its tiles
+  int pre_extra, own_extra;  // places of a unit on the line beside its tiles'
+  int pre_cost;          // places of a prefix tile; an own tile has one
   long long pre_total;   // places of all prefix units
   // workspace
   long long* starts;     // [entries + 1] places before an entry's units
@@ -742,9 +743,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const long long from = cut.first(blockIdx.x), to = cut.first(blockIdx.x + 1);
   auto pre_tiles_before = [&](long long place) -> int {
     if (place <= 0 || p.pre_total == 0) return 0;
-    const int len = p.pre_tiles + p.pre_extra;
+    const int len = p.pre_tiles * p.pre_cost + p.pre_extra;
     const int at = (int)min(place, p.pre_total), unit = at / len;
-    return unit * p.pre_tiles + max(0, at - unit * len - p.pre_extra);
+    return unit * p.pre_tiles + max(0, at - unit * len - p.pre_extra + p.pre_cost - 1) / p.pre_cost;
   };
   Part part;
   part.pre_first = pre_tiles_before(from);
@@ -852,9 +853,10 @@ __global__ void __launch_bounds__(32 * kJoinWarps, kJoinBlocks) join_kernel(cons
     if (p.share) {
       const int row = at.b * p.rows + r;
       pu_e = row / (2 * kTile), pu_r = row % (2 * kTile);
-      pre.stop = ((long long)h * p.pre_row_tiles + pu_e + 1) * (p.pre_tiles + p.pre_extra);
-      pre.start = pre.stop - p.pre_tiles;
-      pc0 = cut.cta_of(pre.start), pc1 = cut.cta_of(pre.stop - 1);
+      pre.stop = ((long long)h * p.pre_row_tiles + pu_e + 1) * (p.pre_tiles * p.pre_cost + p.pre_extra);
+      pre.start = pre.stop - p.pre_tiles * p.pre_cost;
+      // a tile is its first place's
+      pc0 = cut.cta_of(pre.start), pc1 = cut.cta_of(pre.stop - p.pre_cost);
     }
     const int n_pre = 2 * (pc1 - pc0 + 1), n_all = n_pre + 2 * (c1 - c0 + 1);
     for (int base = 0; base < n_all; base += 32) {
@@ -869,7 +871,10 @@ __global__ void __launch_bounds__(32 * kJoinWarps, kJoinBlocks) join_kernel(cons
         const bool wide = is_pre ? p.pre_wide : p.own_wide;
         const long long c_start = cut.first(cta), c_stop = cut.first(cta + 1);
         const int ur = is_pre ? pu_r : r;
-        const bool there = min(u.stop, c_stop) > max(u.start, c_start) && (!wide || (ur >> 7) == s);
+        const int cost = is_pre ? p.pre_cost : 1;
+        const int t0 = (int)(max(u.start, c_start) - u.start + cost - 1) / cost;
+        const int t1 = (int)(min(u.stop, c_stop) - u.start + cost - 1) / cost;
+        const bool there = t1 > t0 && (!wide || (ur >> 7) == s);
         if (there) {
           const long long slot =
               2 * slot_of(p, is_pre, is_pre ? pu_e : e, h, cta, u.start < c_start) + s;
@@ -953,9 +958,12 @@ int64_t make_plan(const sy_attend_args& a, int sms, Plan* p, char* ws) {
   p->pre_row_tiles = p->pre_wide ? (int)((pre_rows + 2 * kTile - 1) / (2 * kTile)) : 1;
   p->own_row_tiles = p->own_wide ? (p->rows + 2 * kTile - 1) / (2 * kTile) : 1;
   p->entries = (int)(a.batch * p->own_row_tiles);
-  p->pre_extra = p->pre_wide ? 2 : 1;
+  // measured: a wide tile takes about twice a narrow one's time, a run of a wide
+  // unit costs about two of its tiles, one of a narrow unit about one
+  p->pre_cost = p->pre_wide ? 2 : 1;
+  p->pre_extra = p->pre_wide ? 4 : 1;
   p->own_extra = p->own_wide ? 2 : 1;
-  p->pre_total = p->share ? (int64_t)(p->pre_tiles + p->pre_extra) * p->pre_row_tiles * a.kv_heads : 0;
+  p->pre_total = p->share ? (int64_t)(p->pre_tiles * p->pre_cost + p->pre_extra) * p->pre_row_tiles * a.kv_heads : 0;
   p->box = (int)(a.page_size & -a.page_size);
   if (p->box > kTile) p->box = kTile;
   p->grid = sms;
