@@ -21,15 +21,15 @@
 // run costs beside its tiles (query rows in, O out, the pipeline's filling).
 //
 // CTA. 12 warps: one loads K and V tiles by TMA through a ring of buffers (the
-// pages' rows land in tile order, so a page may end inside a tile), one issues
-// the MMAs, two gather query rows, and two streams of four warps each own 128
+// pages' rows land in tile order, so a page may end inside a tile), one gathers
+// query rows, two issue MMAs, and two streams of four warps each own 128
 // softmax rows (one row a thread, so no shuffles). S = Q K^T goes to TMEM, a
-// stream reads its row, moves the maximum only when it grew by more than 2^8
-// (then rescales its part of O in TMEM), writes P over S as 16-bit, and P V
+// stream reads its row, moves the maximum only when it grew much (then rescales
+// its part of O in TMEM), writes P over S as 16-bit, and P V
 // accumulates in TMEM with P as the TMEM operand. Units of more than 128 rows
 // give each stream 128 of the rows ("wide": one K/V tile serves 256 rows);
-// smaller ones give both streams the same rows and every second tile, each with
-// its own O and (m, l), so the MMAs of one overlap the softmax of the other.
+// smaller ones give both streams the same rows and half of every tile's keys, each
+// with its own O and (m, l).
 #include <cmath>
 
 #include "sy_common.cuh"
@@ -41,9 +41,9 @@ namespace sy {
 namespace {
 
 constexpr int kTile = 128;     // keys of a tile, rows of a stream
-constexpr int kThreads = 384;  // load, MMA, 2 query warps, 2 x 4 softmax warps
+constexpr int kThreads = 384;  // load, query, 2 MMA warps, 2 streams x 4 softmax warps
+constexpr int kHalf = 64;      // keys of a step of the softmax
 constexpr int kBarBytes = 3072;  // barriers and scratch behind the tiles
-constexpr float kGrow = 8.f;   // log2 of the growth of a maximum that is let pass
 
 struct Plan {
   sy_attend_args a;
@@ -228,13 +228,13 @@ struct Smem {
 
 struct Bars {
   uint64_t full[10], empty[10];
-  uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2];
+  // [stream][buffer of S]; o_done: P V of the step that had this buffer
+  uint64_t q_full[2], q_empty[2], s_full[2][2], p_full[2][2], o_done[2][2];
   uint32_t tmem;
   int run_tiles[2];  // tiles of the run that a query tile belongs to
-  int stop;          // a query warp gave up
   int own_e, own_h, own_off, own_start, own_stop;
   long long scan[kThreads / 32];
-  long long q_at[2 * kTile];  // byte offset of a run's query rows
+  uint32_t q_at[kTile];  // where a query tile's rows start, in 16 bytes
 };
 static_assert(sizeof(Bars) <= kBarBytes, "barriers and scratch");
 
@@ -322,13 +322,13 @@ __device__ __forceinline__ void load_tiles(const Plan& p, const CUtensorMap* kma
 }
 
 // ---- query rows: gathered into the MMA's swizzled layout ----
-// 16 lanes copy a row's 16-byte chunks (fewer than 16 below head_dim 128), four
+// 16 lanes copy a row's 16-byte chunks (fewer than 16 below head_dim 128), two
 // rows a step; where the rows start is worked out once per run.
 template <int DP>
 __device__ __forceinline__ void load_queries(const Plan& p, char* smem, Bars* bars, const Part& part) {
   using S = Smem<DP>;
-  const int tid = threadIdx.x - 64;  // 64 threads
-  const int c = tid & 15, r0 = tid >> 4;
+  const int lane = threadIdx.x & 31;
+  const int c = lane & 15, r0 = lane >> 4;
   const bool on = c < (int)p.a.head_dim / 8;
   const char* q = static_cast<const char*>(p.a.q) + c * 16;
   const uint32_t to = smem_u32(smem) + S::kQ + (c >> 3) * (kTile * 128);
@@ -341,112 +341,123 @@ __device__ __forceinline__ void load_queries(const Plan& p, char* smem, Bars* ba
 #pragma unroll 1
     for (; cur.live(); cur.next_run(p)) {
       const int rows = unit_rows(p, cur.pre, cur.e);
-      named_sync(1, 64);  // the table's readers are done
-#pragma unroll 1
-      for (int r = tid; r < rows; r += 64) {
-        const RowAt at = row_at(p, cur.pre, cur.e, cur.h, r);
-        bars->q_at[r] = 2 * (at.b * p.a.q_b + at.t * p.a.q_t + at.head * p.a.q_h);
-      }
-      named_sync(1, 64);
 #pragma unroll 1
       for (int s = 0; s < (wide ? 2 : 1); ++s, ++slot) {
-        const int buf = slot & 1;
-        if (!warp_wait(&bars->q_empty[buf], ((slot >> 1) & 1) ^ 1)) {
-          bars->stop = 1;  // the other warp must not wait at the barrier alone
+        const int buf = slot & 1, count = min(kTile, rows - s * kTile);
+        if (!warp_wait(&bars->q_empty[buf], ((slot >> 1) & 1) ^ 1)) return;
+#pragma unroll 1
+        for (int r = lane; r < count; r += 32) {
+          const RowAt at = row_at(p, cur.pre, cur.e, cur.h, s * kTile + r);
+          bars->q_at[r] = (uint32_t)((at.b * p.a.q_b + at.t * p.a.q_t + at.head * p.a.q_h) / 8);
         }
-        const int count = min(kTile, rows - s * kTile);
+        __syncwarp();
         if (on)
 #pragma unroll 4
-          for (int r = r0; r < count; r += 4)
+          for (int r = r0; r < count; r += 2)
             cp_async16(to + buf * S::kTileBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4),
-                       q + bars->q_at[s * kTile + r]);
+                       q + 16ll * bars->q_at[r]);
         cp_async_wait_all();
         fence_proxy_async();
         __syncwarp();
-        if ((threadIdx.x & 31) == 0) {
+        if (lane == 0) {
           bars->run_tiles[buf] = cur.j1 - cur.j0;
           mbar_arrive(&bars->q_full[buf]);
         }
       }
-      named_sync(1, 64);
-      if (bars->stop) return;
     }
   }
 }
 
 // ---- MMAs ----
-// One thread. It follows the tiles without knowing the units: the query warps
-// publish every run's length with its query tile.
+// A warp per stream; one elected lane issues. (The loop is the whole warp's, so
+// that the compiler sees uniform values: with one lane in it every descriptor
+// went through vector registers and an MMA took 80 cycles to issue instead of
+// 35. One warp for both streams spent most of its time on waits and commits, one
+// after the other: 4.8k cycles a wide tile against 2.6k of tensor work.)
+// A stream's work is a line of steps of 64 keys: both halves of every tile in a
+// wide unit, half s of every tile in a narrow one. Step n's S goes to buffer
+// n & 1 of the stream, its P to the first columns of that buffer; P V of step n
+// comes before S of step n + 2 in the tensor pipe, which executes in order, so
+// nothing else guards the buffer. The next S is always under way while the
+// softmax is busy with the one before.
+// The warp does not know the units: the query warp publishes every run's length
+// with its query tile.
 struct MmaState {
   int k_stage = 0, v_stage = 1;  // ring buffers of the next K and V tile
   uint32_t k_phase = 0, v_phase = 0;
-  int slot = 0;          // query tiles used up
-  uint32_t p_phase = 0;  // bit s: parity of stream s's next P
+  int slot = 0;          // query tiles used up, by both streams
+  uint32_t p_phase = 0;  // bit b: parity of the next P in buffer b
 };
 
 template <int DP, bool BF16>
-__device__ __forceinline__ bool issue_mmas(uint32_t base, Bars* bars, uint32_t tmem, int count,
+__device__ __forceinline__ bool issue_mmas(uint32_t base, Bars* bars, uint32_t tmem, int s, int count,
                                            bool wide, MmaState& st) {
   using S = Smem<DP>;
-  constexpr uint32_t kIdS = f16_idesc(BF16, kTile, kTile, false);
+  constexpr uint32_t kIdS = f16_idesc(BF16, kTile, kHalf, false);
   constexpr uint32_t kIdO = f16_idesc(BF16, kTile, DP, true);
   const uint64_t q_desc = sw128_desc(base + S::kQ, 16, 1024);
   const uint64_t k_desc = sw128_desc(base + S::kRing, 16, 1024);
   const uint64_t v_desc = sw128_desc(base + S::kRing, kTile * 128, 1024);
-  const int ahead = wide ? 1 : 2;  // tiles that S runs ahead of P V, and between two of a stream
-  int at = 0, run = 0;             // place in the run of the next S tile
-  uint32_t marks = 0;              // tiles j, j + 1, ..: bit 0 first, bit 1 last of a stream's run
-  // step i issues P V of tile i - ahead and S of tile i, stream by stream
+  const int steps = wide ? 2 * count : count;
+  const uint32_t o_at = tmem + (2 + s) * kTile;
+  int at = 0, run = 0;  // place in the run, its length, in steps, of the next S
+  uint32_t fresh = 0;   // bit i: the i-th step between S and P V opens a run
 #pragma unroll 1
-  for (int i = 0; i < count + ahead; ++i) {
-    const int j = i - ahead;
-    if (j >= 0 && !wait(&bars->full[st.v_stage], st.v_phase)) return false;
-    const uint32_t mine = marks;
-    const uint64_t v = v_desc + (uint32_t)(st.v_stage * (S::kTileBytes >> 4));
-#pragma unroll 1
-    for (int s = wide ? 0 : i & 1; s <= (wide ? 1 : i & 1); ++s) {
-      const bool done = !wide || s == 1;  // with this tile's buffers
-      if (j >= 0) {
-        if (!wait(&bars->p_full[s], (st.p_phase >> s) & 1)) return false;
-        st.p_phase ^= 1u << s;
-        tc_fence_after();
+  for (int n = 0; n < steps + 2; ++n) {
+    // a wide unit's tile is done with its second half
+    const bool tile_first = !wide || (n & 1) == 0, tile_last = !wide || (n & 1) == 1;
+    const int half = wide ? n & 1 : s, buf = n & 1;
+    const uint32_t s_at = tmem + s * kTile + buf * kHalf;
+    if (n >= 2) {
+      if (tile_first && !warp_wait(&bars->full[st.v_stage], st.v_phase)) return false;
+      if (!warp_wait(&bars->p_full[s][buf], (st.p_phase >> buf) & 1)) return false;
+      st.p_phase ^= 1u << buf;
+      tc_fence_after();
+      const uint64_t v = v_desc + (uint32_t)((st.v_stage * S::kTileBytes + half * kHalf * 128) >> 4);
+      if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < kTile / 16; ++k)
-          mma_ts(tmem + 2 * kTile + s * kTile, tmem + s * kTile + k * 8,
-                 v + (uint32_t)(k * (2048 >> 4)), kIdO, k > 0 || !(mine & 1u));
-        if (mine & 2u) tc_commit(&bars->o_full[s]);
-        if (done) tc_commit(&bars->empty[st.v_stage]);
+        for (int k = 0; k < kHalf / 16; ++k)
+          mma_ts(o_at, s_at + k * 8, v + (uint32_t)(k * (2048 >> 4)), kIdO, k > 0 || !(fresh & 1u));
+        tc_commit(&bars->o_done[s][buf]);
+        if (tile_last) tc_commit(&bars->empty[st.v_stage]);
       }
-      if (i < count) {
-        const int slot = st.slot + (wide ? s : 0), buf = slot & 1;
-        if (!wait(&bars->full[st.k_stage], st.k_phase)) return false;
-        if (at == 0) {
-          if (!wait(&bars->q_full[buf], (slot >> 1) & 1)) return false;
-          run = bars->run_tiles[buf];
-        }
-        const uint64_t a = q_desc + (uint32_t)(buf * (S::kTileBytes >> 4));
-        const uint64_t b = k_desc + (uint32_t)(st.k_stage * (S::kTileBytes >> 4));
+      __syncwarp();
+      fresh >>= 1;
+      if (tile_last) {
+        st.v_stage += 2;
+        if (st.v_stage >= S::kStages) st.v_stage -= S::kStages, st.v_phase ^= 1;
+      }
+    }
+    if (n < steps) {
+      if (tile_first && !warp_wait(&bars->full[st.k_stage], st.k_phase)) return false;
+      const int slot = st.slot + (wide ? s : 0), q = slot & 1;
+      if (at == 0) {
+        if (!warp_wait(&bars->q_full[q], (slot >> 1) & 1)) return false;
+        run = __shfl_sync(kFull, bars->run_tiles[q], 0) * (wide ? 2 : 1);
+        fresh |= 1u << (n < 2 ? n : 1);
+      }
+      const uint64_t a = q_desc + (uint32_t)(q * (S::kTileBytes >> 4));
+      const uint64_t b = k_desc + (uint32_t)((st.k_stage * S::kTileBytes + half * kHalf * 128) >> 4);
+      const bool run_last = at + 1 == run;
+      if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k) {
           const uint32_t off = ((k >> 2) * (kTile * 128) + (k & 3) * 32) >> 4;
-          mma_ss(tmem + s * kTile, a + off, b + off, kIdS, k > 0);
+          mma_ss(s_at, a + off, b + off, kIdS, k > 0);
         }
-        tc_commit(&bars->s_full[s]);
-        if (at + 1 == run) tc_commit(&bars->q_empty[buf]);
-        if (done) tc_commit(&bars->empty[st.k_stage]);
+        tc_commit(&bars->s_full[s][buf]);
+        if (tile_last) tc_commit(&bars->empty[st.k_stage]);
+        if (run_last) {
+          // a query tile is released by two: both streams, or one of them twice
+          tc_commit(&bars->q_empty[q]);
+          if (wide) tc_commit(&bars->q_empty[q]);
+        }
       }
-    }
-    if (j >= 0) {
-      marks >>= 2;
-      st.v_stage += 2;
-      if (st.v_stage >= S::kStages) st.v_stage -= S::kStages, st.v_phase ^= 1;
-    }
-    if (i < count) {
-      // tile i stands `ahead` places behind the next P V, which is tile j + 1
-      const int place = 2 * (j >= 0 ? ahead - 1 : i);
-      marks |= ((at < ahead ? 1u : 0u) | (run - at <= ahead ? 2u : 0u)) << place;
-      st.k_stage += 2;
-      if (st.k_stage >= S::kStages) st.k_stage -= S::kStages, st.k_phase ^= 1;
+      __syncwarp();
+      if (tile_last) {
+        st.k_stage += 2;
+        if (st.k_stage >= S::kStages) st.k_stage -= S::kStages, st.k_phase ^= 1;
+      }
       if (++at == run) at = 0, st.slot += wide ? 2 : 1;
     }
   }
@@ -467,8 +478,14 @@ __device__ __forceinline__ uint32_t pack16<__half>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// fp16 weights are kept 2^6 higher: they may reach 2^(6 + 8) and lose bits only
-// below 2^-20 of the highest.
+// A row's maximum only moves when a tile exceeds it by more than 2^grow: every
+// move costs a pass over O. Weights are then at most 2^grow, which bf16 and the
+// fp32 sums hold with the same relative precision; fp16 weights are kept 2^6
+// higher, may reach 2^(6 + 8) and lose bits only below 2^-20 of the highest.
+template <typename T>
+__device__ __forceinline__ constexpr float grow() {
+  return std::is_same<T, __half>::value ? 8.f : 32.f;
+}
 template <typename T>
 __device__ __forceinline__ constexpr float weight_shift() {
   return std::is_same<T, __half>::value ? 6.f : 0.f;
@@ -493,6 +510,25 @@ __device__ __forceinline__ float row_max(const uint32_t* x) {
   return fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3]));
 }
 
+// 32 weights 2^(c x + off) from x[0..31]: summed, then rounded to 16 bits into x[0..15]
+template <typename T>
+__device__ __forceinline__ void weights(uint32_t* x, float c, float off, float2& sum0, float2& sum1) {
+  const float2 c2 = make_float2(c, c), off2 = make_float2(off, off);
+#pragma unroll
+  for (int k = 0; k < 32; k += 4) {
+    float2 u = make_float2(__uint_as_float(x[k]), __uint_as_float(x[k + 1]));
+    float2 w = make_float2(__uint_as_float(x[k + 2]), __uint_as_float(x[k + 3]));
+    u = __ffma2_rn(u, c2, off2);
+    w = __ffma2_rn(w, c2, off2);
+    u = make_float2(ex2(u.x), ex2(u.y));
+    w = make_float2(ex2(w.x), ex2(w.y));
+    sum0 = __fadd2_rn(sum0, u);
+    sum1 = __fadd2_rn(sum1, w);
+    x[k / 2] = pack16<T>(u.x, u.y);
+    x[k / 2 + 1] = pack16<T>(w.x, w.y);
+  }
+}
+
 // Where a stream's partial result of a row stands.
 __device__ __forceinline__ long long part_at(const Plan& p, const Cursor& cur, int s, int row) {
   const long long slot = 2 * slot_of(p, cur.pre, cur.e, cur.h, blockIdx.x, cur.first > 0) + s;
@@ -509,7 +545,7 @@ __device__ __forceinline__ void put_rows(const Plan& p, const Cursor& cur, int s
                                          uint32_t o_at, float m, float l) {
   const int row = min((int)threadIdx.x & 127, rows - 1);
   const bool mine = ((int)threadIdx.x & 127) < rows;
-  const bool final = !cur.pre && !p.share && cur.whole() && (wide || cur.n == 1);
+  const bool final = !cur.pre && !p.share && wide && cur.whole();
   const float inv = l > 0.f ? 1.f / l : 0.f;
   char* dst;
   if (final) {
@@ -524,15 +560,15 @@ __device__ __forceinline__ void put_rows(const Plan& p, const Cursor& cur, int s
     if (mine) part_ml(p, cur, s, row) = make_float2(m * p.c, l);
   }
 #pragma unroll 1
-  for (int i = 0; i < DP / 32; ++i) {
+  for (int col = 0; col < DP; col += 32) {
     uint32_t o[32];
-    tmem_ld32(o_at + 32 * i, o);
+    tmem_ld32(o_at + col, o);
     tmem_wait_ld(o);
     if (!mine) continue;
     if (!final) {
 #pragma unroll
       for (int k = 0; k < 32; k += 4)
-        *reinterpret_cast<uint4*>(dst + (32 * i + k) * 4) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+        *reinterpret_cast<uint4*>(dst + (col + k) * 4) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
     } else {
 #pragma unroll
       for (int k = 0; k < 32; k += 8) {
@@ -542,8 +578,8 @@ __device__ __forceinline__ void put_rows(const Plan& p, const Cursor& cur, int s
           const float lo = __uint_as_float(o[k + 2 * u]) * inv, hi = __uint_as_float(o[k + 2 * u + 1]) * inv;
           w[u] = l > 0.f ? pack16<T>(lo, hi) : 0u;
         }
-        if (32 * i + k < (int)p.a.head_dim)
-          *reinterpret_cast<uint4*>(dst + (32 * i + k) * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+        if (col + k < (int)p.a.head_dim)
+          *reinterpret_cast<uint4*>(dst + (col + k) * 2) = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
   }
@@ -555,118 +591,98 @@ __device__ __forceinline__ void softmax_rows(const Plan& p, char* smem, Bars* ba
   using S = Smem<DP>;
   const int row = threadIdx.x & 127, warp = row >> 5;
   const uint32_t lanes = (uint32_t)warp << 21;  // TMEM lane in bits 16..31
-  const uint32_t s_at = tmem + lanes + s * kTile, o_at = tmem + lanes + (2 + s) * kTile;
+  const uint32_t o_at = tmem + lanes + (2 + s) * kTile;
   const float c = p.c;
-  uint32_t s_phase = 0, o_phase = 0;
   int base_pos = 1;  // ring position of the phase's first V tile
+  // bit b: parity of the next S in buffer b; P V of the step before this one has
+  // the parity that its S had. (P V of the step before that is done: this step's
+  // S came after it.)
+  uint32_t phases = 0;
 #pragma unroll 1
   for (int ph = 0; ph < 2; ++ph) {
     Cursor cur;
     cur.start(p, part, ph == 0);
     const bool wide = ph == 0 ? p.pre_wide : p.own_wide;
-    const int step = wide ? 1 : 2;
+    uint32_t buf = 0;  // a phase begins with buffer 0
 #pragma unroll 1
     for (; cur.live(); cur.next_run(p)) {
-      // narrow: tile j of the phase is stream j & 1's
-      const int j_first = wide ? cur.j0 : cur.j0 + ((cur.j0 ^ s) & 1);
       const int rows = unit_rows(p, cur.pre, cur.e) - (wide ? s * kTile : 0);
-      if (j_first >= cur.j1) {  // a run of one tile, the other stream's
-        if (row < rows) part_ml(p, cur, s, row) = make_float2(-INFINITY, 0.f);
-        continue;
-      }
       const bool active = warp * 32 < rows;
       int see = 0;  // own keys that this row sees
       if (!cur.pre)
         see = cur.len - (int)p.a.q_len + 1 +
               row_at(p, false, cur.e, cur.h, (wide ? s * kTile : 0) + max(0, min(row, rows - 1))).t;
       float m = -INFINITY, l = 0.f;
+      const int steps = (cur.j1 - cur.j0) * (wide ? 2 : 1);
 #pragma unroll 1
-      for (int j = j_first; j < cur.j1; j += step) {
+      for (int i = 0; i < steps; ++i, buf ^= 1) {
+        const int half = wide ? i & 1 : s, j = cur.j0 + (wide ? i >> 1 : i);
         const int t = cur.first + j - cur.j0;
         const int keys = cur.keys(p, t);
-        if (!warp_wait(&bars->s_full[s], s_phase)) return;
-        s_phase ^= 1;
+        if (!warp_wait(&bars->s_full[s][buf], (phases >> buf) & 1)) return;
+        phases ^= 1u << buf;
         tc_fence_after();
-        if (active) {
-          const int upto = cur.in_prefix(p, t) ? keys : min(keys, see - cur.key0(p, t));
-          const bool masked = __any_sync(kFull, upto < kTile);
-          float top = -INFINITY;
-          uint32_t x[32];
-          // the row is read twice, 32 columns at a time
-#pragma unroll 1
-          for (int i = 0; i < kTile; i += 32) {
-            tmem_ld32(s_at + i, x);
-            tmem_wait_ld(x);
-            if (masked) mask_columns(x, upto - i);
-            top = fmaxf(top, row_max(x));
-          }
-          // The first maximum is taken as it is; later ones only past 2^kGrow.
-          const bool moves = m == -INFINITY ? top > -INFINITY : (top - m) * c > kGrow;
-          if (__any_sync(kFull, moves)) {
-            const float keep = !moves ? 1.f : m == -INFINITY ? 0.f : ex2((m - top) * c);
-            if (moves) m = top;
-            l *= keep;
-            if (j != j_first) {
-              // S of this tile follows the stream's last P V in the MMA order: O stands still
-#pragma unroll 1
-              for (int i = 0; i < DP / 32; ++i) {
-                tmem_ld32(o_at + 32 * i, x);
-                tmem_wait_ld(x);
-#pragma unroll
-                for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) * keep);
-                tmem_st32(o_at + 32 * i, x);
-              }
-            }
-          }
-          const float off = (m == -INFINITY ? 0.f : -m * c) + weight_shift<T>();
-          const float2 c2 = make_float2(c, c), off2 = make_float2(off, off);
-          float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
-#pragma unroll 1
-          for (int i = 0; i < kTile; i += 32) {
-            tmem_ld32(s_at + i, x);
-            tmem_wait_ld(x);
-            if (masked) mask_columns(x, upto - i);
-#pragma unroll
-            for (int k = 0; k < 32; k += 4) {
-              float2 u = make_float2(__uint_as_float(x[k]), __uint_as_float(x[k + 1]));
-              float2 w = make_float2(__uint_as_float(x[k + 2]), __uint_as_float(x[k + 3]));
-              u = __ffma2_rn(u, c2, off2);
-              w = __ffma2_rn(w, c2, off2);
-              u = make_float2(ex2(u.x), ex2(u.y));
-              w = make_float2(ex2(w.x), ex2(w.y));
-              sum0 = __fadd2_rn(sum0, u);
-              sum1 = __fadd2_rn(sum1, w);
-              x[k / 2] = pack16<T>(u.x, u.y);
-              x[k / 2 + 1] = pack16<T>(w.x, w.y);
-            }
-            tmem_st16(s_at + i / 2, x);  // P takes the first half of S's columns, already read
-          }
-          l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
-          tmem_wait_st();
-        }
-        if (keys < kTile) {
+        if (keys < kTile && (!wide || half == 0)) {
           // What lies behind the last key in its page may be anything, and 0 * NaN
-          // is NaN: clear V there. Both streams of a wide unit do, each before its
-          // own P V.
+          // is NaN: clear V there, every warp before it gives its weights away.
           const int vpos = base_pos + 2 * j, stage = vpos % S::kStages;
           if (!warp_wait(&bars->full[stage], (vpos / S::kStages) & 1)) return;
           char* v = smem + S::kRing + stage * S::kTileBytes + keys * 128;
 #pragma unroll 1
-          for (int i = row; i < (kTile - keys) * 8; i += 128)
+          for (int z = row; z < (kTile - keys) * 8; z += 128)
 #pragma unroll
-            for (int half = 0; half < DP / 64; ++half)
-              *reinterpret_cast<uint4*>(v + half * (kTile * 128) + i * 16) = make_uint4(0, 0, 0, 0);
+            for (int d = 0; d < DP / 64; ++d)
+              *reinterpret_cast<uint4*>(v + d * (kTile * 128) + z * 16) = make_uint4(0, 0, 0, 0);
           fence_proxy_async();
+        }
+        if (active) {
+          const uint32_t s_at = tmem + lanes + s * kTile + buf * kHalf;
+          const int upto = (cur.in_prefix(p, t) ? keys : min(keys, see - cur.key0(p, t))) - kHalf * half;
+          uint32_t x[kHalf];
+          tmem_ld32(s_at, x);
+          tmem_ld32(s_at + 32, x + 32);
+          tmem_wait_ld(x);
+          tmem_landed(x + 32);
+          if (__any_sync(kFull, upto < kHalf)) mask_columns(x, upto), mask_columns(x + 32, upto - 32);
+          const float top = fmaxf(row_max(x), row_max(x + 32));
+          // The first maximum is taken as it is; later ones only past 2^grow.
+          const bool moves = m == -INFINITY ? top > -INFINITY : top > m + grow<T>() / c;
+          if (__any_sync(kFull, moves)) {
+            const float keep = !moves ? 1.f : m == -INFINITY ? 0.f : ex2((m - top) * c);
+            if (moves) m = top;
+            l *= keep;
+            if (i > 0) {
+              // O stands still once the last P V is done: the next needs this step's weights
+              if (!warp_wait(&bars->o_done[s][buf ^ 1], (~phases >> (buf ^ 1)) & 1)) return;
+              tc_fence_after();
+#pragma unroll 1
+              for (int col = 0; col < DP; col += 32) {
+                uint32_t o[32];
+                tmem_ld32(o_at + col, o);
+                tmem_wait_ld(o);
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
+                tmem_st32(o_at + col, o);
+              }
+            }
+          }
+          const float off = (m == -INFINITY ? 0.f : -m * c) + weight_shift<T>();
+          float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
+          weights<T>(x, c, off, sum0, sum1);
+          tmem_st16(s_at, x);  // P takes the first half of its S
+          weights<T>(x + 32, c, off, sum0, sum1);
+          tmem_st16(s_at + 16, x + 32);
+          l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
+          tmem_wait_st();
         }
         tc_fence_before();
         __syncwarp();
-        if ((threadIdx.x & 31) == 0) mbar_arrive(&bars->p_full[s]);
+        if ((threadIdx.x & 31) == 0) mbar_arrive(&bars->p_full[s][buf]);
       }
-      if (!warp_wait(&bars->o_full[s], o_phase)) return;
-      o_phase ^= 1;
+      if (!warp_wait(&bars->o_done[s][buf ^ 1], (~phases >> (buf ^ 1)) & 1)) return;
       tc_fence_after();
       if (active) put_rows<T, DP>(p, cur, s, wide, rows, o_at, m, l);
-      tc_fence_before();  // the next run's P V overwrites O after the next p_full
+      tc_fence_before();  // the next run's P V overwrites O after the next weights
     }
     base_pos += 2 * cur.end;
   }
@@ -685,7 +701,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ __align__(1024) char smem[];
   Bars* bars = reinterpret_cast<Bars*>(smem + S::kBars);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(kFull, tid >> 5, 0);
   pdl_trigger();
   if (smem_u32(smem) & 1023u) {  // the swizzle and the descriptors count on it
     if (tid == 0) record_device_error(kDevErrBadPlan);
@@ -715,17 +732,19 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
     for (int i = 0; i < S::kStages; ++i) {
       mbar_init(&bars->full[i], 1);
-      mbar_init(&bars->empty[i], 1);
+      mbar_init(&bars->empty[i], 2);
     }
 #pragma unroll 1
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bars->q_full[i], 2);
-      mbar_init(&bars->q_empty[i], 1);
-      mbar_init(&bars->s_full[i], 1);
-      mbar_init(&bars->p_full[i], 4);
-      mbar_init(&bars->o_full[i], 1);
+      mbar_init(&bars->q_full[i], 1);
+      mbar_init(&bars->q_empty[i], 2);
+#pragma unroll 1
+      for (int k = 0; k < 2; ++k) {
+        mbar_init(&bars->s_full[i][k], 1);
+        mbar_init(&bars->o_done[i][k], 1);
+        mbar_init(&bars->p_full[i][k], 4);
+      }
     }
-    bars->stop = 0;
     mbar_fence_init();
     tma_prefetch_map(&kmap);
     tma_prefetch_map(&vmap);
@@ -777,7 +796,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (blockIdx.x == 0 && tid == kThreads - 1) p.starts[p.entries] = total - p.pre_total;
   __syncthreads();
   part.own_e = bars->own_e, part.own_h = bars->own_h, part.own_off = bars->own_off;
-  part.own_count = own_to > own_from ? bars->own_stop - bars->own_start : 0;
+  part.own_count = __shfl_sync(kFull, own_to > own_from ? bars->own_stop - bars->own_start : 0, 0);
+  part.pre_count = __shfl_sync(kFull, part.pre_count, 0);
   if (part.pre_count + part.own_count == 0) return;
 
   if (warp == 2) tmem_alloc(&bars->tmem, 512);
@@ -787,22 +807,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = bars->tmem;
+  const uint32_t tmem = __shfl_sync(kFull, bars->tmem, 0);
 
   if (warp == 0) {
     load_tiles<DP>(p, &kmap, &vmap, smem, bars, part);
   } else if (warp == 1) {
-    if (lane == 0) {
-      MmaState st;
-      bool ok = true;
-#pragma unroll 1
-      for (int ph = 0; ok && ph < 2; ++ph)
-        ok = issue_mmas<DP, kBf16>(smem_u32(smem), bars, tmem, ph ? part.own_count : part.pre_count,
-                                   ph ? p.own_wide : p.pre_wide, st);
-    }
-    __syncwarp();
-  } else if (warp < 4) {
     load_queries<DP>(p, smem, bars, part);
+  } else if (warp < 4) {
+    MmaState st;
+    bool ok = true;
+#pragma unroll 1
+    for (int ph = 0; ok && ph < 2; ++ph)
+      ok = issue_mmas<DP, kBf16>(smem_u32(smem), bars, tmem, warp - 2,
+                                 ph ? part.own_count : part.pre_count, ph ? p.own_wide : p.pre_wide, st);
   } else {
     softmax_rows<T, DP>(p, smem, bars, tmem, warp >= 8, part);
   }
@@ -839,7 +856,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps, kJoinBlocks) join_kernel(cons
   const int n = (int)(own.stop - own.start);
   const Cut cut(total, p.grid);
   const int c0 = n ? cut.cta_of(own.start) : 0, c1 = n ? cut.cta_of(own.stop - 1) : -1;
-  if (!p.share && n && c0 == c1 && (p.own_wide || n == 1)) return;  // already written
+  if (!p.share && n && c0 == c1 && p.own_wide) return;  // already written
   const int rows = unit_rows(p, false, e);
   const float ln2 = 0.69314718055994531f;
   for (int r = r0 + warp; r < min(rows, r0 + kJoinRows); r += kJoinWarps) {

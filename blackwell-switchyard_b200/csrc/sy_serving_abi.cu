@@ -64,7 +64,15 @@ int check_attend(const sy_attend_args* a, bool pointers) {
   const int64_t strides[] = {a->q_b,     a->q_t,    a->q_h,     a->kc_page, a->kc_head,
                              a->kc_row, a->vc_page, a->vc_head, a->vc_row};
   for (int64_t s : strides)
-    if (s < 0 || s % 8 != 0) return SY_ERR_ARG;
+    if (s < 0 || s % 8 != 0 || s > (int64_t(1) << 38)) return SY_ERR_ARG;
+  // the kernel counts the start of a query row in 32 bits, in units of 16 bytes
+  int64_t reach = 0;
+  const int64_t steps[3][2] = {{a->batch, a->q_b}, {a->q_len, a->q_t}, {a->q_heads, a->q_h}};
+  for (const auto& s : steps) {
+    if (s[0] > 1 && s[1] > (int64_t(1) << 35) / (s[0] - 1)) return SY_ERR_UNSUPPORTED;
+    reach += (s[0] - 1) * s[1];
+  }
+  if (reach >= int64_t(1) << 35) return SY_ERR_UNSUPPORTED;
   return SY_OK;
 }
 

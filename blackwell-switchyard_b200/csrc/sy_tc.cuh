@@ -8,6 +8,15 @@
 
 namespace sy {
 
+// One lane of a converged warp, the same one every time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+
 // ---------------------------------------------------------------------------
 // TMEM allocation (one warp, all lanes; columns a power of two >= 32)
 // ---------------------------------------------------------------------------
