@@ -61,9 +61,9 @@ struct Plan {
   int pre_slot_rows, own_slot_rows;
   int pre_extra, own_extra;  // places of a unit on the line beside its tiles'
   int pre_cost;          // places of a prefix tile; an own tile has one
-  long long pre_total;   // places of all prefix units
+  int pre_total;         // places of all prefix units
   // workspace
-  long long* starts;     // [entries + 1] places before an entry's units
+  int* starts;           // [entries + 1] places before an entry's units
   float *pre_ml, *pre_o, *own_ml, *own_o;
 };
 
@@ -87,19 +87,15 @@ __device__ __forceinline__ int entry_tiles(const Plan& p, int lim) {
 // places of a unit of n tiles; its tiles are the last n of them
 __device__ __forceinline__ int own_places(const Plan& p, int n) { return n > 0 ? n + p.own_extra : 0; }
 
-// The line's cut: CTA c has the places [first(c), first(c + 1)).
+// The line's cut: CTA c has the places [first(c), first(c + 1)). (The host
+// checked that the line is shorter than 2^31.)
 struct Cut {
-  long long total;
-  int grid;
-  long long q;  // total = q grid + rem
-  int rem;
-  __device__ __forceinline__ Cut(long long t, int g) : total(t), grid(g), q(t / g), rem((int)(t % g)) {}
-  __device__ __forceinline__ long long first(int c) const { return q * c + rem * c / grid; }
-  __device__ __forceinline__ int cta_of(long long place) const {
-    int c = min(grid - 1, (int)((float)place * (float)grid / (float)total));
-    while (first(c) > place) --c;
-    while (first(c + 1) <= place) ++c;
-    return c;
+  int q, rem;  // the first rem CTAs have q + 1 places, the others q
+  __device__ __forceinline__ Cut(int total, int grid) : q(total / grid), rem(total - q * grid) {}
+  __device__ __forceinline__ int first(int c) const { return q * c + min(c, rem); }
+  __device__ __forceinline__ int cta_of(int place) const {
+    const int big = rem * (q + 1);
+    return place < big ? place / (q + 1) : rem + (place - big) / q;
   }
 };
 
@@ -750,28 +746,28 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_map(&vmap);
   }
   __syncthreads();
-  long long total = 0;
+  long long sums = 0;
 #pragma unroll 1
   for (int w = 0; w < kThreads / 32; ++w) {
     if (w < warp) upto += bars->scan[w];
-    total += bars->scan[w];
+    sums += bars->scan[w];
   }
   const int heads = (int)p.a.kv_heads;
-  total = (total & 0xffffffffll) * heads + p.pre_total;
+  const int total = (int)(sums & 0xffffffffll) * heads + p.pre_total;
   const Cut cut(total, p.grid);
-  const long long from = cut.first(blockIdx.x), to = cut.first(blockIdx.x + 1);
-  auto pre_tiles_before = [&](long long place) -> int {
+  const int from = cut.first(blockIdx.x), to = cut.first(blockIdx.x + 1);
+  auto pre_tiles_before = [&](int place) -> int {
     if (place <= 0 || p.pre_total == 0) return 0;
     const int len = p.pre_tiles * p.pre_cost + p.pre_extra;
-    const int at = (int)min(place, p.pre_total), unit = at / len;
+    const int at = min(place, p.pre_total), unit = at / len;
     return unit * p.pre_tiles + max(0, at - unit * len - p.pre_extra + p.pre_cost - 1) / p.pre_cost;
   };
   Part part;
   part.pre_first = pre_tiles_before(from);
   part.pre_count = pre_tiles_before(to) - part.pre_first;
   // The own part's ends: the thread whose entries they fall into works them out.
-  const long long own_from = max(from, p.pre_total) - p.pre_total, own_to = to - p.pre_total;
-  long long before = ((upto - mine) & 0xffffffffll) * heads, tiles = ((upto - mine) >> 32) * heads;
+  const int own_from = max(from, p.pre_total) - p.pre_total, own_to = to - p.pre_total;
+  int before = (int)((upto - mine) & 0xffffffffll) * heads, tiles = (int)((upto - mine) >> 32) * heads;
 #pragma unroll 1
   for (int e = e_first; e < e_last; ++e) {
     const int b = e / p.own_row_tiles;
@@ -780,18 +776,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (blockIdx.x == 0) p.starts[e] = before;
 #pragma unroll 1
     for (int end = 0; end < 2; ++end) {
-      const long long rel = (end ? own_to : own_from) - before;
-      if (rel < end || rel >= (long long)len * heads + end) continue;
-      const int h = (int)(rel - end) / len, off = max(0, (int)(rel - (long long)h * len) - p.own_extra);
+      const int rel = (end ? own_to : own_from) - before;
+      if (rel < end || rel >= len * heads + end) continue;
+      const int h = (rel - end) / len, off = max(0, rel - h * len - p.own_extra);
       if (end) {
-        bars->own_stop = (int)(tiles + (long long)h * n + off);
+        bars->own_stop = tiles + h * n + off;
       } else {
         bars->own_e = e, bars->own_h = h, bars->own_off = off;
-        bars->own_start = (int)(tiles + (long long)h * n + off);
+        bars->own_start = tiles + h * n + off;
       }
     }
-    before += (long long)len * heads;
-    tiles += (long long)n * heads;
+    before += len * heads;
+    tiles += n * heads;
   }
   if (blockIdx.x == 0 && tid == kThreads - 1) p.starts[p.entries] = total - p.pre_total;
   __syncthreads();
@@ -833,114 +829,135 @@ __global__ void __launch_bounds__(kThreads, 1)
 // ---------------------------------------------------------------------------
 // The places of a unit's tiles.
 struct Places {
-  long long start, stop;
+  int start, stop;
 };
 
-constexpr int kJoinWarps = 8, kJoinRows = 16, kJoinBlocks = 5;  // blocks an SM
+constexpr int kJoinWarps = 8;
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(32 * kJoinWarps, kJoinBlocks) join_kernel(const Plan p) {
-  pdl_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// A warp joins R rows. 32 / R lanes a row look at the runs that may hold a part
+// of it (an online softmax over them); the whole warp then adds the parts up, a
+// lane having four columns of each row, with 8 loads in flight. Units of many
+// rows have few runs (R = 4), units of few rows many (R = 1).
+template <typename T, int DP, int R>
+__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_constant__ Plan p) {
+  constexpr int kLanes = 32 / R, kAtOnce = 8 / R;
+  const int lane = threadIdx.x & 31, sub = lane % kLanes;
   const int unit_max = p.own_wide ? min(p.rows, 2 * kTile) : p.rows;
-  const int groups = (unit_max + kJoinRows - 1) / kJoinRows;
+  const int groups = (unit_max + R - 1) / R;
   const int heads = (int)p.a.kv_heads;
-  const long long block = blockIdx.x;
-  const int e = (int)(block / groups / heads), h = (int)(block / groups % heads);
-  const int r0 = (int)(block % groups) * kJoinRows;
-  const long long own_total = p.starts[p.entries], total = own_total + p.pre_total;
-  const int places = (int)(p.starts[e + 1] - p.starts[e]) / heads;
-  Places own;
-  own.stop = p.pre_total + p.starts[e] + (h + 1ll) * places;
+  const int group = blockIdx.x * kJoinWarps + (threadIdx.x >> 5);
+  const int unit = group / groups;
+  const int e = unit / heads, h = unit - e * heads;
+  if (e >= p.entries) return;
+  const int rows = unit_rows(p, false, e), r = (group - unit * groups) * R + lane / kLanes;
+  pdl_wait();
+  const int own_at = p.starts[e], places = (p.starts[e + 1] - own_at) / heads;
+  const Cut cut(p.starts[p.entries] + p.pre_total, p.grid);
+  Places own, pre;
+  own.stop = p.pre_total + own_at + (h + 1) * places;
   own.start = own.stop - places + (places ? p.own_extra : 0);
-  const int n = (int)(own.stop - own.start);
-  const Cut cut(total, p.grid);
-  const int c0 = n ? cut.cta_of(own.start) : 0, c1 = n ? cut.cta_of(own.stop - 1) : -1;
-  if (!p.share && n && c0 == c1 && p.own_wide) return;  // already written
-  const int rows = unit_rows(p, false, e);
-  const float ln2 = 0.69314718055994531f;
-  for (int r = r0 + warp; r < min(rows, r0 + kJoinRows); r += kJoinWarps) {
-    const RowAt at = row_at(p, false, e, h, r);
-    const long long out_row = (at.b * p.a.q_len + at.t) * p.a.q_heads + at.head;
-    float m = -INFINITY, l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    // candidates: (CTA, stream) of the prefix unit, then of the own unit
-    int pu_e = 0, pu_r = 0, pc0 = 0, pc1 = -1;
-    Places pre = own;
-    if (p.share) {
-      const int row = at.b * p.rows + r;
-      pu_e = row / (2 * kTile), pu_r = row % (2 * kTile);
-      pre.stop = ((long long)h * p.pre_row_tiles + pu_e + 1) * (p.pre_tiles * p.pre_cost + p.pre_extra);
-      pre.start = pre.stop - p.pre_tiles * p.pre_cost;
-      // a tile is its first place's
-      pc0 = cut.cta_of(pre.start), pc1 = cut.cta_of(pre.stop - p.pre_cost);
-    }
-    const int n_pre = 2 * (pc1 - pc0 + 1), n_all = n_pre + 2 * (c1 - c0 + 1);
-    for (int base = 0; base < n_all; base += 32) {
-      const int i = base + lane;
-      float cm = -INFINITY, cl = 0.f;
-      long long at_row = 0;
+  const bool any = own.stop > own.start;
+  const int c0 = any ? cut.cta_of(own.start) : 0, c1 = any ? cut.cta_of(own.stop - 1) : -1;
+  if (!p.share && any && c0 == c1 && p.own_wide) return;  // already written
+  const bool mine = r < rows;
+  const RowAt at = row_at(p, false, e, h, mine ? r : 0);
+  const long long out_row = (at.b * p.a.q_len + at.t) * p.a.q_heads + at.head;
+  // candidates: (CTA, stream) of the prefix unit, then of the own unit
+  int pu_e = 0, pu_r = 0, pc0 = 0, pc1 = -1;
+  pre = own;
+  if (p.share) {
+    const int row = at.b * p.rows + (mine ? r : 0);
+    pu_e = row / (2 * kTile), pu_r = row - pu_e * 2 * kTile;
+    pre.stop = (h * p.pre_row_tiles + pu_e + 1) * (p.pre_tiles * p.pre_cost + p.pre_extra);
+    pre.start = pre.stop - p.pre_tiles * p.pre_cost;
+    // a tile is its first place's
+    pc0 = cut.cta_of(pre.start), pc1 = cut.cta_of(pre.stop - p.pre_cost);
+  }
+  const int n_pre = 2 * (pc1 - pc0 + 1), n_all = mine ? n_pre + 2 * (c1 - c0 + 1) : 0;
+  float m = -INFINITY, l = 0.f;
+  float4 o[R];
+#pragma unroll
+  for (int k = 0; k < R; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+  for (int i = sub; __any_sync(kFull, i - sub < n_all); i += kLanes) {
+    float cm = -INFINITY, cl = 0.f;
+    const float* src = p.own_o;
+    if (i < n_all) {
       const bool is_pre = i < n_pre;
-      if (i < n_all) {
-        const int k = is_pre ? i : i - n_pre;
-        const int cta = (is_pre ? pc0 : c0) + (k >> 1), s = k & 1;
-        const Places& u = is_pre ? pre : own;
-        const bool wide = is_pre ? p.pre_wide : p.own_wide;
-        const long long c_start = cut.first(cta), c_stop = cut.first(cta + 1);
-        const int ur = is_pre ? pu_r : r;
-        const int cost = is_pre ? p.pre_cost : 1;
-        const int t0 = (int)(max(u.start, c_start) - u.start + cost - 1) / cost;
-        const int t1 = (int)(min(u.stop, c_stop) - u.start + cost - 1) / cost;
-        const bool there = t1 > t0 && (!wide || (ur >> 7) == s);
-        if (there) {
-          const long long slot =
-              2 * slot_of(p, is_pre, is_pre ? pu_e : e, h, cta, u.start < c_start) + s;
-          at_row = slot * (is_pre ? p.pre_slot_rows : p.own_slot_rows) + (wide ? ur & 127 : ur);
-          const float2 ml = reinterpret_cast<const float2*>(is_pre ? p.pre_ml : p.own_ml)[at_row];
-          if (ml.y > 0.f) cm = ml.x, cl = ml.y;
-        }
+      const int k = is_pre ? i : i - n_pre;
+      const int cta = (is_pre ? pc0 : c0) + (k >> 1), s = k & 1;
+      const int start = is_pre ? pre.start : own.start, stop = is_pre ? pre.stop : own.stop;
+      const int from = max(start, cut.first(cta)) - start, to = min(stop, cut.first(cta + 1)) - start;
+      // tiles whose first place lies in [from, to); a prefix tile has pre_cost (1 or 2) places
+      const int up = is_pre ? p.pre_cost - 1 : 0;
+      const bool wide = is_pre ? p.pre_wide : p.own_wide;
+      const int ur = is_pre ? pu_r : r;
+      if (((to + up) >> up) > ((from + up) >> up) && (!wide || (ur >> 7) == s)) {
+        const long long slot = 2 * slot_of(p, is_pre, is_pre ? pu_e : e, h, cta, from > 0) + s;
+        const long long at_row = slot * (is_pre ? p.pre_slot_rows : p.own_slot_rows) + (wide ? ur & 127 : ur);
+        const float2 ml = reinterpret_cast<const float2*>(is_pre ? p.pre_ml : p.own_ml)[at_row];
+        src = (is_pre ? p.pre_o : p.own_o) + at_row * DP;
+        if (ml.y > 0.f) cm = ml.x, cl = ml.y;
       }
-      const float top = fmaxf(m, warp_max(cm));
-      if (top == -INFINITY) continue;
-      const float keep = m == -INFINITY ? 0.f : ex2(m - top);
-      const float w = cm == -INFINITY ? 0.f : ex2(cm - top);
-      m = top;
-      l = l * keep + warp_sum(w * cl);
-      o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
-      const float* src = (is_pre ? p.pre_o : p.own_o) + at_row * DP;
-      unsigned live = __ballot_sync(kFull, w > 0.f);
-      while (live) {
-        constexpr int kAtOnce = 4;
-        float4 x[kAtOnce];
-        float f[kAtOnce];
-        unsigned rest = live;
+    }
+    float top = fmaxf(m, cm);
 #pragma unroll
-        for (int k = 0; k < kAtOnce; ++k) {
-          const int from = rest ? __ffs(rest) - 1 : 0;
-          f[k] = __shfl_sync(kFull, w, from);
+    for (int x = 1; x < kLanes; x <<= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, x));
+    const float keep = m == -INFINITY ? 0.f : ex2(m - top);
+    const float w = cm == -INFINITY ? 0.f : ex2(cm - top);
+    m = top;
+    float add = w * cl;
+#pragma unroll
+    for (int x = 1; x < kLanes; x <<= 1) add += __shfl_xor_sync(kFull, add, x);
+    l = l * keep + add;
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      const float f = __shfl_sync(kFull, keep, kLanes * k);
+      o[k].x *= f, o[k].y *= f, o[k].z *= f, o[k].w *= f;
+    }
+    unsigned live = __ballot_sync(kFull, w > 0.f);
+#pragma unroll
+    for (int x = kLanes; x < 32; x <<= 1) live |= live >> x;  // candidates live in any row
+    if (kLanes < 32) live &= (1u << (kLanes & 31)) - 1u;
+#pragma unroll 1
+    while (live) {
+      float4 x[kAtOnce][R];
+      float f[kAtOnce][R];
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        const int j = live ? __ffs(live) - 1 : 0;
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+          f[u][k] = __shfl_sync(kFull, w, kLanes * k + j);
           const float* ptr = reinterpret_cast<const float*>(
-              __shfl_sync(kFull, reinterpret_cast<unsigned long long>(src), from));
-          if (!rest) f[k] = 0.f;
-          x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (rest && lane * 4 < DP) x[k] = __ldcs(reinterpret_cast<const float4*>(ptr) + lane);
-          rest &= rest - 1;
+              __shfl_sync(kFull, reinterpret_cast<unsigned long long>(src), kLanes * k + j));
+          if (!live) f[u][k] = 0.f;
+          x[u][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (f[u][k] > 0.f && lane * 4 < DP) x[u][k] = __ldcs(reinterpret_cast<const float4*>(ptr) + lane);
         }
-#pragma unroll
-        for (int k = 0; k < kAtOnce; ++k) {
-          o.x += f[k] * x[k].x, o.y += f[k] * x[k].y;
-          o.z += f[k] * x[k].z, o.w += f[k] * x[k].w;
-        }
-        live = rest;
+        live &= live - 1;
       }
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+          o[k].x += f[u][k] * x[u][k].x, o[k].y += f[u][k] * x[u][k].y;
+          o[k].z += f[u][k] * x[u][k].z, o[k].w += f[u][k] * x[u][k].w;
+        }
     }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    if (lane * 4 < (int)p.a.head_dim) {
-      T* out = static_cast<T*>(p.a.out) + out_row * p.a.head_dim + lane * 4;
-      *reinterpret_cast<uint2*>(out) =
-          make_uint2(pack16<T>(o.x * inv, o.y * inv), pack16<T>(o.z * inv, o.w * inv));
-    }
-    if (lane == 0 && p.a.lse)
-      p.a.lse[out_row] = l > 0.f ? m * ln2 + logf(l) - weight_shift<T>() * ln2 : -INFINITY;
+  }
+  const float ln2 = 0.69314718055994531f;
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  if (mine && sub == 0 && p.a.lse)
+    p.a.lse[out_row] = l > 0.f ? (m - weight_shift<T>()) * ln2 + logf(l) : -INFINITY;
+#pragma unroll
+  for (int k = 0; k < R; ++k) {
+    const float f = __shfl_sync(kFull, inv, kLanes * k);
+    const long long row = __shfl_sync(kFull, out_row, kLanes * k);
+    const bool put = __shfl_sync(kFull, (int)mine, kLanes * k);
+    if (put && lane * 4 < (int)p.a.head_dim)
+      *reinterpret_cast<uint2*>(static_cast<T*>(p.a.out) + row * p.a.head_dim + lane * 4) =
+          make_uint2(pack16<T>(o[k].x * f, o[k].y * f), pack16<T>(o[k].z * f, o[k].w * f));
   }
 }
 
@@ -957,9 +974,11 @@ __global__ void __launch_bounds__(256) no_keys_kernel(const sy_attend_args a) {
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
+constexpr int64_t kMaxLine = int64_t(1) << 31;
+
 int64_t align16(int64_t x) { return (x + 15) / 16 * 16; }
 
-// Fills everything but the pointers into the workspace; returns its bytes.
+// Fills the plan, its pointers from `ws` on; returns the workspace's bytes, or -status.
 int64_t make_plan(const sy_attend_args& a, int sms, Plan* p, char* ws) {
   p->a = a;
   const int dp = a.head_dim > 64 ? 128 : 64;
@@ -980,7 +999,14 @@ int64_t make_plan(const sy_attend_args& a, int sms, Plan* p, char* ws) {
   p->pre_cost = p->pre_wide ? 2 : 1;
   p->pre_extra = p->pre_wide ? 4 : 1;
   p->own_extra = p->own_wide ? 2 : 1;
-  p->pre_total = p->share ? (int64_t)(p->pre_tiles * p->pre_cost + p->pre_extra) * p->pre_row_tiles * a.kv_heads : 0;
+  const int64_t pre_line =
+      p->share ? ((int64_t)p->pre_tiles * p->pre_cost + p->pre_extra) * p->pre_row_tiles * a.kv_heads : 0;
+  const int64_t own_line =
+      (p->lead_tiles + (a.table_width * a.page_size + kTile - 1) / kTile + p->own_extra) * a.kv_heads;
+  // the kernels count places in 32 bits
+  if (pre_line >= kMaxLine || own_line >= kMaxLine || own_line * p->entries >= kMaxLine - pre_line)
+    return -SY_ERR_UNSUPPORTED;
+  p->pre_total = (int)pre_line;
   p->box = (int)(a.page_size & -a.page_size);
   if (p->box > kTile) p->box = kTile;
   p->grid = sms;
@@ -997,7 +1023,7 @@ int64_t make_plan(const sy_attend_args& a, int sms, Plan* p, char* ws) {
     at += align16(bytes);
     return q;
   };
-  p->starts = reinterpret_cast<long long*>(take((p->entries + 1) * 8));
+  p->starts = reinterpret_cast<int*>(take((p->entries + 1) * 4));
   p->pre_ml = reinterpret_cast<float*>(take(pre_slots * 8));
   p->own_ml = reinterpret_cast<float*>(take(own_slots * 8));
   p->pre_o = reinterpret_cast<float*>(take(pre_slots * dp * 4));
@@ -1046,9 +1072,11 @@ cudaError_t launch_type(const Plan& p, const CUtensorMap& k, const CUtensorMap& 
                               k, v);
   if (e != cudaSuccess) return e;
   const int unit_max = p.own_wide ? (p.rows < 2 * kTile ? p.rows : 2 * kTile) : p.rows;
-  const int64_t groups = (unit_max + kJoinRows - 1) / kJoinRows;
-  return launch_smem_pdl(join_kernel<T, DP>, dim3((unsigned)(p.entries * p.a.kv_heads * groups)),
-                         32 * kJoinWarps, 0, st, p);
+  const int each = unit_max >= kTile ? 4 : 1;
+  const int64_t warps = (int64_t)p.entries * p.a.kv_heads * ((unit_max + each - 1) / each);
+  const dim3 grid((unsigned)((warps + kJoinWarps - 1) / kJoinWarps));
+  return each == 4 ? launch_smem_pdl(join_kernel<T, DP, 4>, grid, 32 * kJoinWarps, 0, st, p)
+                   : launch_smem_pdl(join_kernel<T, DP, 1>, grid, 32 * kJoinWarps, 0, st, p);
 }
 
 }  // namespace

@@ -115,7 +115,9 @@ int sy_attend(const sy_attend_args* args, sy_stream_t stream) {
   sy::ServingDev dev;
   const cudaError_t e = sy::serving_dev(&dev);
   if (e != cudaSuccess) return sy::cuda_error_status(e, "sy_attend");
-  if (args->workspace_bytes < sy::attend_workspace(*args, dev) ||
+  const int64_t need = sy::attend_workspace(*args, dev);
+  if (need < 0) return (int)-need;
+  if (args->workspace_bytes < need ||
       (args->workspace_bytes > 0 && (!args->workspace || !sy::al16(args->workspace))))
     return SY_ERR_ARG;
   return sy::cuda_error_status(sy::launch_attend(*args, dev, static_cast<cudaStream_t>(stream)),
