@@ -10,13 +10,16 @@
 // one 64-bit number, their rank key; "the first k" and "the first with weight
 // p Z" are then "every rank key from some cut on". To find a cut, all tokens are
 // counted and weighed in 2048 bins of equal width in max - x (weights beyond
-// 28.4 are zero); the bin that holds the cut has a few tokens, as a rule, which
+// 28.4 are zero), at first only in the quarter next to the maximum, as a cut
+// rarely lies deeper and most tokens do; the bin that holds the cut has a few tokens, as a rule, which
 // are gathered and ranked by comparing all pairs. A bin with more than kList of
 // them (ties, flat rows) is cut by eight radix passes over the rank keys instead.
 // The draw then adds the kept weights in index order: CTAs, warps, lanes.
 //
 // The row's bytes are the floor for many rows (256 x 131071 fp32: 20.5 us at the
-// measured copy rate); for one row it is a chain of about ten cluster barriers.
+// measured copy rate); for one row it is a chain of six to nine cluster barriers.
+// A remote shared-memory read costs as much as a barrier, so CTAs push what others
+// need (maxima, sums, the leader's verdicts) ahead of the barrier and read locally.
 #include <cooperative_groups.h>
 
 #include <cmath>
@@ -37,21 +40,34 @@ constexpr int kBins = 2048, kList = 1024;
 constexpr int kMaxCluster = 8;
 constexpr float kSpan = 28.43f;                      // exp(-kSpan) 2^40 rounds to 0
 constexpr float kBinsPer = (kBins - 1) / kSpan;      // bins per unit of max - x
+constexpr int kNear = 512;                           // bins filled at first: 7.1 below the maximum
 constexpr int64_t kMaxSlice = 128 * 1024;            // bytes of a slice in shared memory
+
+// What the leader found, pushed to every CTA.
+struct Verdict {
+  u64 cut;        // kept so far: rank keys from here on
+  u64 goal;       // weight of p_bin from its top to the cut
+  int k_bin;      // the bin that top_k cuts, kBins if none
+  int p_bin;      // the bin that top_p cuts, kBins if none (or not known before top_k's cut)
+  unsigned need;  // tokens of k_bin up to the cut
+  int enough;     // the bins filled so far hold the cuts
+};
 
 struct State {
   u64 wbin[kBins];       // weight per bin
   unsigned cbin[kBins];  // tokens per bin
-  u64 list[kList], sorted[kList];
-  unsigned listed;
-  float max_x;
-  unsigned max_at;
-  u64 total;             // this CTA's kept weight
-  // what the leader found, read by the others
-  int bin;
-  unsigned need;         // tokens (or 0: weight) of the bin up to the cut
-  u64 goal, cut;
-  u64 red[kWarps];
+  u64 list[2][kList];    // rank keys gathered for top_k's and top_p's cut
+  u64 sorted[kList];     // also the radix passes' bins
+  unsigned listed[2];
+  Verdict verdict;
+  // one per CTA of the cluster, pushed
+  float max_x[kMaxCluster];
+  unsigned max_at[kMaxCluster];
+  u64 sums[kMaxCluster], kept[kMaxCluster];
+  u64 found, upto;       // leader: a cut, and the weight up to and with it
+  u64 goal_above;        // leader: weight above the radix passes' prefix
+  unsigned left;
+  u64 red[2][kWarps];
   float fred[kWarps];
   unsigned ured[kWarps];
 };
@@ -72,8 +88,22 @@ __device__ __forceinline__ float x_of(u64 rank) {
 __device__ __forceinline__ float mass_of(float x, float top) {
   return x == top ? 1.f : expf(__fsub_rn(x, top));
 }
+// rint(2^40 e). Below 2^23 adding 2^23 rounds to a whole number and leaves it in
+// the low bits; from there on the float is whole and its mantissa is shifted. (The
+// 64-bit conversion instruction has a small fraction of this rate.)
 __device__ __forceinline__ u64 weight_of(float e) {
-  return __float2ull_rn(__fmul_rn(e, 1099511627776.f));  // 2^40
+  const float y = __fmul_rn(e, 1099511627776.f);
+  if (y < 8388608.f) return __float_as_uint(__fadd_rn(y, 8388608.f)) - 0x4b000000u;
+  const unsigned b = __float_as_uint(y);
+  return (u64)((b & 0x7fffffu) | 0x800000u) << ((b >> 23) - 150u);
+}
+// Add to a 64-bit sum in shared memory by 32-bit atomics, which the hardware has:
+// whoever wraps the low word carries.
+__device__ __forceinline__ void add_weight(u64* sum, u64 w) {
+  unsigned* word = reinterpret_cast<unsigned*>(sum);
+  const unsigned lo = (unsigned)w, old = atomicAdd(word, lo);
+  const unsigned hi = (unsigned)(w >> 32) + (old + lo < old ? 1u : 0u);
+  if (hi) atomicAdd(word + 1, hi);
 }
 // the bin of x, or kBins where the weight is zero
 __device__ __forceinline__ int bin_of(float x, float top) {
@@ -86,34 +116,31 @@ __device__ __forceinline__ u64 warp_sum64(u64 x) {
   for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(kFull, x, o);
   return x;
 }
-__device__ __forceinline__ u64 block_sum64(u64 x, u64* red) {
-  x = warp_sum64(x);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = x;
-  __syncthreads();
-  u64 s = 0;
-#pragma unroll 4
-  for (int w = 0; w < kWarps; ++w) s += red[w];
-  return s;
-}
-// exclusive prefix over the block
-__device__ __forceinline__ u64 block_before64(u64 x, u64* red) {
+// Exclusive prefixes over the block of two values at a time; `all` gets the totals.
+__device__ __forceinline__ void block_before(const u64 (&x)[2], u64 (&before)[2], u64 (&all)[2],
+                                             u64 (*red)[kWarps]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  u64 y = x;
+  u64 y[2] = {x[0], x[1]};
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const u64 z = __shfl_up_sync(kFull, y, o);
-    if (lane >= o) y += z;
+    const u64 a = __shfl_up_sync(kFull, y[0], o), b = __shfl_up_sync(kFull, y[1], o);
+    if (lane >= o) y[0] += a, y[1] += b;
   }
   __syncthreads();
-  if (lane == 31) red[warp] = y;
+  if (lane == 31) red[0][warp] = y[0], red[1][warp] = y[1];
   __syncthreads();
-  u64 before = y - x;
-#pragma unroll 4
-  for (int w = 0; w < kWarps; ++w)
-    if (w < warp) before += red[w];
-  return before;
+  // each half of the warp adds up one value's sums
+  u64 w = red[lane >> 4][lane & 15];
+  u64 mine = (lane & 15) < warp ? w : 0;
+#pragma unroll
+  for (int o = 8; o; o >>= 1) w += __shfl_xor_sync(kFull, w, o), mine += __shfl_xor_sync(kFull, mine, o);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    all[i] = __shfl_sync(kFull, w, 16 * i);
+    before[i] = y[i] - x[i] + __shfl_sync(kFull, mine, 16 * i);
+  }
 }
+static_assert(kWarps == 16, "block_before: one value's sums are half a warp's lanes");
 
 template <typename T>
 struct Slice {
@@ -164,62 +191,47 @@ __device__ __forceinline__ void read_slice(const Slice<T>& s, float& top, unsign
   if (tail < s.count) see(tail, p[tail]);
 }
 
-// Gather the rank keys of a bin into the leader's list. Returns their number.
-template <typename T>
-__device__ __forceinline__ unsigned gather(cg::cluster_group& cluster, State* st, State* lead,
-                                           const Slice<T>& s, float top, int bin) {
-  if (cluster.block_rank() == 0 && threadIdx.x == 0) st->listed = 0;
-  cluster.sync();
+// The cut inside a bin from its gathered rank keys: the need-th or, with need == 0,
+// the first at which the weight from the bin's top reaches goal. The leader's block
+// only; the results are st->found and st->upto, valid after the block's barrier here.
+__device__ __forceinline__ void rank_list(State* st, const u64* list, unsigned n, unsigned need, u64 goal,
+                                          float top) {
+  for (unsigned i = threadIdx.x; i < n; i += kThreads) {
+    const u64 mine = list[i];
+    unsigned rank = 0;
 #pragma unroll 4
-  for (unsigned i = threadIdx.x; i < s.count; i += kThreads) {
-    const float x = s.at(i);
-    if (bin_of(x, top) == bin) {
-      const unsigned at = atomicAdd(&lead->listed, 1u);
-      if (at < kList) lead->list[at] = rank_key(x, s.first + i);
-    }
+    for (unsigned j = 0; j < n; ++j) rank += list[j] > mine;
+    st->sorted[rank] = mine;
   }
-  cluster.sync();
-  return lead->listed;
+  __syncthreads();
+  const unsigned a = 2 * threadIdx.x, b = a + 1;
+  const u64 wa = a < n ? weight_of(mass_of(x_of(st->sorted[a]), top)) : 0;
+  const u64 wb = b < n ? weight_of(mass_of(x_of(st->sorted[b]), top)) : 0;
+  const u64 x[2] = {wa + wb, 0};
+  u64 before[2], all[2];
+  block_before(x, before, all, st->red);
+  const u64 ua = before[0] + wa, ub = ua + wb;
+  if (a < n && (need ? a + 1 == need : before[0] < goal && ua >= goal)) st->found = st->sorted[a], st->upto = ua;
+  if (b < n && (need ? b + 1 == need : ua < goal && ub >= goal)) st->found = st->sorted[b], st->upto = ub;
+  __syncthreads();
 }
 
-// The cut inside `bin`: the rank key of its need-th token or, with need == 0, of
-// the first at which the weight from the bin's top reaches goal. `upto` gets the
-// weight up to and with the cut. All CTAs of the cluster call it together; the
-// results are valid in all.
+// The same for a bin with too many tokens for a list: eight radix passes over the
+// rank keys, highest digit first, by the whole cluster into the leader's bins.
 template <typename T>
-__device__ __forceinline__ void cut_bin(cg::cluster_group& cluster, State* st, State* lead,
-                                        const Slice<T>& s, float top, int bin, unsigned need, u64 goal,
-                                        u64& cut, u64& upto) {
-  const unsigned n = gather(cluster, st, lead, s, top, bin);
-  if (n <= kList) {
-    if (cluster.block_rank() == 0) {
-      for (unsigned i = threadIdx.x; i < n; i += kThreads) {
-        const u64 mine = st->list[i];
-        unsigned rank = 0;
-#pragma unroll 4
-        for (unsigned j = 0; j < n; ++j) rank += st->list[j] > mine;
-        st->sorted[rank] = mine;
-      }
-      __syncthreads();
-      const unsigned a = 2 * threadIdx.x, b = a + 1;
-      const u64 wa = a < n ? weight_of(mass_of(x_of(st->sorted[a]), top)) : 0;
-      const u64 wb = b < n ? weight_of(mass_of(x_of(st->sorted[b]), top)) : 0;
-      const u64 before = block_before64(wa + wb, st->red);
-      const u64 ua = before + wa, ub = ua + wb;
-      if (a < n && (need ? a + 1 == need : before < goal && ua >= goal)) st->cut = st->sorted[a], st->goal = ua;
-      if (b < n && (need ? b + 1 == need : ua < goal && ub >= goal)) st->cut = st->sorted[b], st->goal = ub;
-    }
-    cluster.sync();
-    cut = lead->cut, upto = lead->goal;
-    cluster.sync();  // before the leader's words are written again
-    return;
-  }
-  // radix passes over the rank key, eight bits at a time, highest digit first
+__device__ __noinline__ void radix_cut(State* st, const Slice<T>& s, float top, int bin, unsigned need,
+                                       u64 goal) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const bool leads = cluster.block_rank() == 0;
+  State* lead = cluster.map_shared_rank(st, 0);
+  u64* wsum = lead->sorted;
+  unsigned* csum = reinterpret_cast<unsigned*>(lead->sorted + 256);
   u64 prefix = 0, above = 0;
   unsigned left = need;
 #pragma unroll 1
   for (int shift = 56; shift >= 0; shift -= 8) {
-    for (int i = threadIdx.x; i < 256; i += kThreads) st->wbin[i] = 0, st->cbin[i] = 0;
+    if (leads)
+      for (int i = threadIdx.x; i < 256; i += kThreads) wsum[i] = 0, csum[i] = 0;
     cluster.sync();
     const u64 mask = shift == 56 ? 0 : ~0ull << (shift + 8);
 #pragma unroll 1
@@ -229,28 +241,28 @@ __device__ __forceinline__ void cut_bin(cg::cluster_group& cluster, State* st, S
       const u64 k = rank_key(x, s.first + i);
       if ((k ^ prefix) & mask) continue;
       const int d = (int)(k >> shift) & 255;
-      atomicAdd(&lead->cbin[d], 1u);
-      atomicAdd(&lead->wbin[d], weight_of(mass_of(x, top)));
+      atomicAdd(&csum[d], 1u);
+      atomicAdd(&wsum[d], weight_of(mass_of(x, top)));
     }
     cluster.sync();
-    if (cluster.block_rank() == 0 && threadIdx.x == 0) {
+    if (leads && threadIdx.x == 0) {
       u64 w = above;
       unsigned c = 0;
       int d = 255;
+#pragma unroll 1
       for (; d > 0; --d) {
-        if (need ? c + st->cbin[d] >= left : w + st->wbin[d] >= goal) break;
-        c += st->cbin[d], w += st->wbin[d];
+        if (need ? c + csum[d] >= left : w + wsum[d] >= goal) break;
+        c += csum[d], w += wsum[d];
       }
-      st->cut = prefix | (u64)d << shift;
-      st->need = left - c;
-      st->goal = w;
-      st->total = w + st->wbin[d];
+      st->found = prefix | (u64)d << shift;
+      st->left = left - c;
+      st->goal_above = w;
+      st->upto = w + wsum[d];
     }
     cluster.sync();
-    prefix = lead->cut, left = lead->need, above = lead->goal, upto = lead->total;
+    prefix = lead->found, left = lead->left, above = lead->goal_above;
     cluster.sync();
   }
-  cut = prefix;
 }
 
 template <typename T>
@@ -260,12 +272,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   State* st = reinterpret_cast<State*>(smem);
   cg::cluster_group cluster = cg::this_cluster();
   const unsigned rank = cluster.block_rank(), ctas = cluster.num_blocks();
+  const bool leads = rank == 0;
   State* lead = cluster.map_shared_rank(st, 0);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const long long r = blockIdx.x / ctas;
   const unsigned V = (unsigned)a.vocab;
   const float temp = a.temperature ? a.temperature[r] : 1.f;
   const bool greedy = !(temp > 0.f);
+  const long long k = greedy ? 1 : a.top_k ? a.top_k[r] : 0;
+  const float p = a.top_p ? a.top_p[r] : 1.f;
+  const float min_p = fminf(a.min_p ? a.min_p[r] : 0.f, 1.f);
+  const float u = a.u[r];
+  const bool by_count = k > 0 && k < V, by_weight = p < 1.f;
 
   Slice<T> s;
   s.row = static_cast<const T*>(a.logits) + r * a.logits_row;
@@ -277,133 +295,199 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   // the maximum and its lowest index
   float top;
   unsigned at;
-  read_slice(s, top, at);
-  if (at != 0xffffffffu) at += s.first;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
+  auto best = [&](int o) {
     const float y = __shfl_xor_sync(kFull, top, o);
     const unsigned i = __shfl_xor_sync(kFull, at, o);
     if (y > top || (y == top && i < at)) top = y, at = i;
-  }
+  };
+  read_slice(s, top, at);
+  if (at != 0xffffffffu) at += s.first;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) best(o);
   if (lane == 0) st->fred[warp] = top, st->ured[warp] = at;
   for (int i = tid; i < kBins; i += kThreads) st->wbin[i] = 0, st->cbin[i] = 0;
+  if (tid < 2) st->listed[tid] = 0;
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < kWarps; ++w)
-      if (st->fred[w] > top || (st->fred[w] == top && st->ured[w] < at)) top = st->fred[w], at = st->ured[w];
-    st->max_x = top, st->max_at = at;
+  if (warp == 0) {
+    top = st->fred[lane & 15], at = st->ured[lane & 15];
+#pragma unroll
+    for (int o = 8; o; o >>= 1) best(o);
+    if (lane < ctas) {
+      State* to = cluster.map_shared_rank(st, lane);
+      to->max_x[rank] = top, to->max_at[rank] = at;
+    }
   }
   cluster.sync();
-  top = -INFINITY, at = 0xffffffffu;
-  for (unsigned c = 0; c < ctas; ++c) {
-    const State* o = cluster.map_shared_rank(st, c);
-    if (o->max_x > top || (o->max_x == top && o->max_at < at)) top = o->max_x, at = o->max_at;
-  }
+  top = lane < ctas ? st->max_x[lane] : -INFINITY, at = lane < ctas ? st->max_at[lane] : 0xffffffffu;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) best(o);
 
-  const long long k = greedy ? 1 : a.top_k ? a.top_k[r] : 0;
-  const float p = a.top_p ? a.top_p[r] : 1.f;
   if (top == -INFINITY || k == 1) {
     // nothing to draw from, or one token: its share is the whole
-    if (rank == 0 && tid == 0) {
+    if (leads && tid == 0) {
       const bool none = top == -INFINITY;
       a.token[r] = none ? -1 : (long long)at;
       if (a.logprob) a.logprob[r] = none ? NAN : 0.f;
     }
-    cluster.sync();  // the others may still be reading this CTA's maximum
-    return;
+    return;  // nobody reads or writes another CTA's memory after the barrier above
   }
 
   u64 cut = 0;  // kept: rank keys from the cut on
-  const bool by_count = k > 0 && k < V, by_weight = p < 1.f;
   if (by_count || by_weight) {
+    // Fill bins [b0, b1) and bring the cluster's together in the leader's; the
+    // first time also add up all weights.
+    auto fill = [&](int b0, int b1) {
+      u64 sum = 0;
 #pragma unroll 4
-    for (unsigned i = tid; i < s.count; i += kThreads) {
-      const float x = s.at(i);
-      const int b = bin_of(x, top);
-      if (b < kBins) {
-        atomicAdd(&st->cbin[b], 1u);
-        if (by_weight) atomicAdd(&st->wbin[b], weight_of(mass_of(x, top)));
-      }
-    }
-    cluster.sync();
-    if (rank) {
-      for (int i = tid; i < kBins; i += kThreads)
-        if (st->cbin[i]) {
-          atomicAdd(&lead->cbin[i], st->cbin[i]);
-          if (by_weight) atomicAdd(&lead->wbin[i], st->wbin[i]);
+      for (unsigned i = tid; i < s.count; i += kThreads) {
+        const float x = s.at(i);
+        const int b = bin_of(x, top);
+        const bool in = b >= b0 && b < b1;
+        if (by_count && in) atomicAdd(&st->cbin[b], 1u);
+        if (by_weight && (in || (b0 == 0 && b < kBins))) {
+          const u64 w = weight_of(mass_of(x, top));
+          sum += w;
+          if (in) add_weight(&st->wbin[b], w);
         }
-    }
-    cluster.sync();
-    // The leader's threads have four bins each: counts and weights before them.
-    constexpr int kEach = kBins / kThreads;
-    u64 c_before = 0, w_before = 0, z = 0;
-    if (rank == 0) {
-      u64 c = 0, w = 0;
+      }
+      if (b0 == 0) {
+        const u64 x[2] = {sum, 0};
+        u64 before[2], all[2];
+        block_before(x, before, all, st->red);
+        if (tid == 0) lead->sums[rank] = all[0];
+      }
+      cluster.sync();
+      if (leads) {
+#pragma unroll 1
+        for (int b = b0 + tid; b < b1; b += kThreads) {
+          u64 w[kMaxCluster];
+          unsigned c[kMaxCluster];
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) c += st->cbin[tid * kEach + i], w += st->wbin[tid * kEach + i];
-      c_before = block_before64(c, st->red);
-      w_before = block_before64(w, st->red);
-      z = block_sum64(w, st->red);
-      if (tid == 0) st->bin = kBins;
+          for (unsigned o = 1; o < kMaxCluster; ++o) {
+            const State* other = cluster.map_shared_rank(st, o < ctas ? o : 0);
+            w[o] = o < ctas ? other->wbin[b] : 0, c[o] = o < ctas ? other->cbin[b] : 0;
+          }
+          w[0] = st->wbin[b], c[0] = st->cbin[b];
+#pragma unroll
+          for (unsigned o = 1; o < kMaxCluster; ++o) w[0] += w[o], c[0] += c[o];
+          st->wbin[b] = w[0], st->cbin[b] = c[0];
+        }
+        __syncthreads();
+      }
+    };
+    // The leader's threads have four bins each; tokens and weight before them.
+    constexpr int kEach = kBins / kThreads;
+    u64 before[2], z = 0;
+    // The bin where the weight reaches p of z (the last one allowed at the latest).
+    auto find_weight = [&](int last) {
+      const double g = ceil((double)fmaxf(p, 0.f) * (double)z);
+      u64 goal = g < 1.0 ? 1ull : (u64)g;
+      if (goal > z) goal = z;
+      u64 weight = before[1];
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int b = tid * kEach + i;
+        if (b <= last && weight < goal && (weight + st->wbin[b] >= goal || b == last))
+          st->verdict.p_bin = b, st->verdict.goal = goal - weight;
+        weight += st->wbin[b];
+      }
+    };
+    auto push_verdict = [&] {  // leader: to every CTA
       __syncthreads();
-      if (by_count) {
-        u64 seen = c_before, weight = w_before;
+      constexpr int kWords = sizeof(Verdict) / 4;
+      if (tid < kWords * (int)(ctas - 1))
+        reinterpret_cast<unsigned*>(&cluster.map_shared_rank(st, 1 + tid / kWords)->verdict)[tid % kWords] =
+            reinterpret_cast<unsigned*>(&st->verdict)[tid % kWords];
+    };
+    u64 ahead = 0;  // leader: weight before top_k's bin
+    auto judge = [&](bool all_filled) {
+      u64 x[2] = {0, 0}, sums[2];
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) x[0] += st->cbin[tid * kEach + i], x[1] += st->wbin[tid * kEach + i];
+      block_before(x, before, sums, st->red);
+      z = lane < ctas ? st->sums[lane] : 0;
+      z = warp_sum64(z);
+      // enough, if k tokens were counted, or the weight that p asks for at most
+      const double g = ceil((double)fmaxf(p, 0.f) * (double)z);
+      const bool enough = all_filled || (by_count ? sums[0] >= (u64)k : (double)sums[1] >= g);
+      if (tid == 0) {
+        st->verdict.enough = enough;
+        st->verdict.k_bin = st->verdict.p_bin = kBins;
+        st->verdict.cut = 0;
+      }
+      __syncthreads();
+      if (enough && by_count) {
+        u64 seen = before[0], weight = before[1];
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
           const int b = tid * kEach + i;
           if (seen < (u64)k && seen + st->cbin[b] >= (u64)k)
-            st->bin = b, st->need = (unsigned)((u64)k - seen), st->goal = weight;
+            st->verdict.k_bin = b, st->verdict.need = (unsigned)((u64)k - seen), st->upto = weight;
           seen += st->cbin[b], weight += st->wbin[b];
         }
-      }
-    }
-    cluster.sync();
-    int last = lead->bin;  // the bin that top_k cuts
-    unsigned need = lead->need;
-    u64 ahead = lead->goal;  // weight before it
-    cluster.sync();
-    if (last < kBins) {
-      // cut_bin's radix passes use the first bins' words: keep the leader's copy
-      u64 keep_w = 0;
-      unsigned keep_c = 0;
-      if (rank == 0 && tid < 256) keep_w = st->wbin[tid], keep_c = st->cbin[tid];
-      u64 upto;
-      cut_bin(cluster, st, lead, s, top, last, need, 0ull, cut, upto);
-      __syncthreads();
-      if (rank == 0 && tid < 256) st->wbin[tid] = keep_w, st->cbin[tid] = keep_c;
-      __syncthreads();
-      z = ahead + upto;
-    }
-    if (by_weight) {
-      if (rank == 0) {
-        const double g = ceil((double)fmaxf(p, 0.f) * (double)z);
-        u64 goal = g < 1.0 ? 1ull : (u64)g;
-        if (goal > z) goal = z;
-        if (tid == 0) st->bin = last;
         __syncthreads();
-        u64 weight = w_before;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-          const int b = tid * kEach + i;
-          if (b <= last && weight < goal && (weight + st->wbin[b] >= goal || b == last))
-            st->bin = b, st->goal = goal - weight;
-          weight += st->wbin[b];
+        ahead = st->upto;
+      }
+      if (enough && by_weight && st->verdict.k_bin == kBins) find_weight(kBins);
+      push_verdict();
+    };
+    fill(0, kNear);
+    if (leads) judge(false);
+    cluster.sync();
+    if (!st->verdict.enough) {
+      fill(kNear, kBins);
+      if (leads) judge(true);
+      cluster.sync();
+    }
+#pragma unroll 1
+    for (int which = 0; which < 2; ++which) {
+      const int bin = which ? st->verdict.p_bin : st->verdict.k_bin;
+      if (bin == kBins) continue;
+      const unsigned need = which ? 0u : st->verdict.need;
+      const u64 goal = which ? st->verdict.goal : 0ull;
+      // gather the bin's rank keys into the leader's list
+#pragma unroll 4
+      for (unsigned i = tid; i < s.count; i += kThreads) {
+        const float x = s.at(i);
+        if (bin_of(x, top) == bin) {
+          const unsigned n = atomicAdd(&lead->listed[which], 1u);
+          if (n < kList) lead->list[which][n] = rank_key(x, s.first + i);
         }
       }
       cluster.sync();
-      const int bin = lead->bin;
-      const u64 goal = lead->goal;
-      cluster.sync();
-      if (bin < kBins) {
-        u64 upto, c;
-        cut_bin(cluster, st, lead, s, top, bin, 0u, goal, c, upto);
-        cut = c > cut ? c : cut;
+      const unsigned n = lead->listed[which];
+      if (n > kList) radix_cut(st, s, top, bin, need, goal);
+      if (leads) {
+        if (n <= kList) rank_list(st, st->list[which], n, need, goal, top);
+        const u64 found = st->found, upto = st->upto;
+        __syncthreads();
+        if (tid == 0) {
+          if (found > st->verdict.cut) st->verdict.cut = found;
+          st->verdict.p_bin = kBins;
+        }
+        if (which == 0 && by_weight) {
+          z = ahead + upto;
+          __syncthreads();
+          find_weight(bin);
+          __syncthreads();
+          if (st->verdict.p_bin == bin && n <= kList) {  // the same bin: its list is here
+            const u64 rest = st->verdict.goal;
+            __syncthreads();
+            rank_list(st, st->list[0], n, 0u, rest, top);
+            if (tid == 0) {
+              if (st->found > st->verdict.cut) st->verdict.cut = st->found;
+              st->verdict.p_bin = kBins;
+            }
+          }
+        }
+        push_verdict();
       }
+      cluster.sync();
     }
+    cut = st->verdict.cut;
   }
 
   // The kept weight, warp by warp in index order.
-  const float min_p = fminf(a.min_p ? a.min_p[r] : 0.f, 1.f);
   const float low = cut ? x_of(cut) : -INFINITY;
   auto kept = [&](unsigned i) -> u64 {
     const float x = s.at(i);
@@ -417,24 +501,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
 #pragma unroll 4
   for (unsigned i = w_first + lane; i < w_last; i += 32) sum += kept(i);
   sum = warp_sum64(sum);
-  __syncthreads();
-  if (lane == 0) st->red[warp] = sum;
-  __syncthreads();
-  u64 before = 0, mine = 0;
-#pragma unroll 4
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += st->red[w];
-    mine += st->red[w];
-  }
-  if (tid == 0) st->total = mine;
-  cluster.sync();
-  u64 total = 0;
-  for (unsigned c = 0; c < ctas; ++c) {
-    const u64 t = cluster.map_shared_rank(st, c)->total;
-    if (c < rank) before += t;
-    total += t;
-  }
-  const double g = floor((double)a.u[r] * (double)total);
+  const u64 x[2] = {lane == 0 ? sum : 0, 0};
+  u64 ahead[2], all[2];
+  block_before(x, ahead, all, st->red);
+  if (tid < (int)ctas) cluster.map_shared_rank(st, tid)->kept[rank] = all[0];
+  cluster.sync();  // the last one: nothing remote is touched after it
+  u64 total = lane < ctas ? st->kept[lane] : 0;
+  u64 before = lane < rank ? total : 0;
+  total = warp_sum64(total);
+  before = warp_sum64(before) + __shfl_sync(kFull, ahead[0], 0);
+  const double g = floor((double)u * (double)total);
   u64 aim = g > 0.0 ? (u64)g : 0ull;
   if (aim >= total) aim = total - 1;
   // the warp whose part holds the aim walks it
@@ -445,8 +521,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       u64 upto = w;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const u64 z = __shfl_up_sync(kFull, upto, o);
-        if (lane >= o) upto += z;
+        const u64 y = __shfl_up_sync(kFull, upto, o);
+        if (lane >= o) upto += y;
       }
       upto += before;
       if (w && upto > aim && upto - w <= aim) {
@@ -457,7 +533,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       if (before > aim) break;
     }
   }
-  cluster.sync();  // no CTA ends while another reads its words
 }
 
 template <typename T>
