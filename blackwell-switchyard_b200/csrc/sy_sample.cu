@@ -72,6 +72,8 @@ struct State {
   unsigned ured[kWarps];
 };
 
+constexpr size_t kStateBytes = (sizeof(State) + 15) / 16 * 16;
+
 // x as an order-preserving 32-bit number; the rank key adds the index, lowest first
 __device__ __forceinline__ unsigned key_of(float x) {
   const unsigned b = __float_as_uint(x + 0.f);  // -0 ranks with +0
@@ -142,35 +144,37 @@ __device__ __forceinline__ void block_before(const u64 (&x)[2], u64 (&before)[2]
 }
 static_assert(kWarps == 16, "block_before: one value's sums are half a warp's lanes");
 
-template <typename T>
+template <typename T, bool Resident>
 struct Slice {
   const T* row;
-  float* x;      // shared memory, or nullptr
+  float* x;  // Resident: the slice's scaled logits in shared memory
   unsigned first, count;
   float inv_t;
   __device__ __forceinline__ float scaled(T v) const {
     const float y = __fmul_rn(Dt<T>::to_f(v), inv_t);
     return y == y ? y : -INFINITY;
   }
-  __device__ __forceinline__ float at(unsigned i) const { return x ? x[i] : scaled(row[first + i]); }
+  __device__ __forceinline__ float at(unsigned i) const {
+    return Resident ? x[i] : scaled(row[first + i]);
+  }
 };
 
-// Read the slice: the maximum and its lowest place; x goes to shared memory.
-template <typename T>
-__device__ __forceinline__ void read_slice(const Slice<T>& s, float& top, unsigned& at) {
+// Read the slice and return its maximum; x goes to shared memory.
+template <typename T, bool Resident>
+__device__ __forceinline__ float read_slice(Slice<T, Resident>& s) {
   constexpr int VEC = 16 / (int)sizeof(T);
-  top = -INFINITY;
-  at = 0xffffffffu;
-  auto see = [&](unsigned i, T v) {
-    const float y = s.scaled(v);
-    if (s.x) s.x[i] = y;
-    if (y > top || (y == top && i < at)) top = y, at = i;
-  };
+  float top = -INFINITY;
   const T* p = s.row + s.first;
   // to the first 16-byte boundary, then whole chunks, four in flight, then the rest
   const unsigned head =
       min(s.count, (unsigned)((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / (unsigned)sizeof(T));
-  if (threadIdx.x < head) see(threadIdx.x, p[threadIdx.x]);
+  s.x += (4 - head) & 3;  // so that the chunks' values are stored 16 bytes at a time
+  auto see = [&](unsigned i) {
+    const float y = s.scaled(p[i]);
+    if (Resident) s.x[i] = y;
+    top = fmaxf(top, y);
+  };
+  if (threadIdx.x < head) see(threadIdx.x);
   const unsigned chunks = (s.count - head) / VEC;
   const uint4* q = reinterpret_cast<const uint4*>(p + head);
 #pragma unroll 1
@@ -183,12 +187,19 @@ __device__ __forceinline__ void read_slice(const Slice<T>& s, float& top, unsign
     for (int u = 0; u < 4; ++u)
       if (c + u * kThreads < chunks) {
         const T* e = reinterpret_cast<const T*>(&v[u]);
+        float y[VEC];
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) see(head + (c + u * kThreads) * VEC + k, e[k]);
+        for (int k = 0; k < VEC; ++k) y[k] = s.scaled(e[k]), top = fmaxf(top, y[k]);
+        if (Resident)
+#pragma unroll
+          for (int k = 0; k < VEC; k += 4)
+            *reinterpret_cast<float4*>(s.x + head + (c + u * kThreads) * VEC + k) =
+                make_float4(y[k], y[k + 1], y[k + 2], y[k + 3]);
       }
   }
   const unsigned tail = head + chunks * VEC + threadIdx.x;
-  if (tail < s.count) see(tail, p[tail]);
+  if (tail < s.count) see(tail);
+  return top;
 }
 
 // The cut inside a bin from its gathered rank keys: the need-th or, with need == 0,
@@ -218,8 +229,8 @@ __device__ __forceinline__ void rank_list(State* st, const u64* list, unsigned n
 
 // The same for a bin with too many tokens for a list: eight radix passes over the
 // rank keys, highest digit first, by the whole cluster into the leader's bins.
-template <typename T>
-__device__ __noinline__ void radix_cut(State* st, const Slice<T>& s, float top, int bin, unsigned need,
+template <typename T, bool Resident>
+__device__ __noinline__ void radix_cut(State* st, const Slice<T, Resident>& s, float top, int bin, unsigned need,
                                        u64 goal) {
   cg::cluster_group cluster = cg::this_cluster();
   const bool leads = cluster.block_rank() == 0;
@@ -265,9 +276,9 @@ __device__ __noinline__ void radix_cut(State* st, const Slice<T>& s, float top, 
   }
 }
 
-template <typename T>
+template <typename T, bool Resident>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_constant__ sy_sample_args a,
-                                                             unsigned slice, bool resident) {
+                                                             unsigned slice) {
   extern __shared__ __align__(16) char smem[];
   State* st = reinterpret_cast<State*>(smem);
   cg::cluster_group cluster = cg::this_cluster();
@@ -285,70 +296,71 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   const float u = a.u[r];
   const bool by_count = k > 0 && k < V, by_weight = p < 1.f;
 
-  Slice<T> s;
+  Slice<T, Resident> s;
   s.row = static_cast<const T*>(a.logits) + r * a.logits_row;
   s.first = min(V, rank * slice);
   s.count = min(V, (rank + 1) * slice) - s.first;
-  s.x = resident ? reinterpret_cast<float*>(smem + sizeof(State)) : nullptr;
+  s.x = reinterpret_cast<float*>(smem + kStateBytes);
   s.inv_t = greedy ? 1.f : __fdiv_rn(1.f, temp);
 
-  // the maximum and its lowest index
-  float top;
-  unsigned at;
-  auto best = [&](int o) {
-    const float y = __shfl_xor_sync(kFull, top, o);
-    const unsigned i = __shfl_xor_sync(kFull, at, o);
-    if (y > top || (y == top && i < at)) top = y, at = i;
-  };
-  read_slice(s, top, at);
-  if (at != 0xffffffffu) at += s.first;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) best(o);
-  if (lane == 0) st->fred[warp] = top, st->ured[warp] = at;
+  float top = warp_max(read_slice(s));
+  if (lane == 0) st->fred[warp] = top;
   for (int i = tid; i < kBins; i += kThreads) st->wbin[i] = 0, st->cbin[i] = 0;
   if (tid < 2) st->listed[tid] = 0;
   __syncthreads();
   if (warp == 0) {
-    top = st->fred[lane & 15], at = st->ured[lane & 15];
-#pragma unroll
-    for (int o = 8; o; o >>= 1) best(o);
-    if (lane < ctas) {
-      State* to = cluster.map_shared_rank(st, lane);
-      to->max_x[rank] = top, to->max_at[rank] = at;
-    }
+    top = warp_max(st->fred[lane & 15]);
+    if (lane < ctas) cluster.map_shared_rank(st, lane)->max_x[rank] = top;
   }
   cluster.sync();
-  top = lane < ctas ? st->max_x[lane] : -INFINITY, at = lane < ctas ? st->max_at[lane] : 0xffffffffu;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) best(o);
+  top = warp_max(lane < ctas ? st->max_x[lane] : -INFINITY);
 
   if (top == -INFINITY || k == 1) {
-    // nothing to draw from, or one token: its share is the whole
-    if (leads && tid == 0) {
-      const bool none = top == -INFINITY;
-      a.token[r] = none ? -1 : (long long)at;
-      if (a.logprob) a.logprob[r] = none ? NAN : 0.f;
+    // nothing to draw from, or one token, the first with the maximum: its share is the whole
+    unsigned at = 0xffffffffu;
+    if (top > -INFINITY)
+#pragma unroll 4
+      for (unsigned i = tid; i < s.count; i += kThreads)
+        if (s.at(i) == top) at = min(at, s.first + i);
+    at = __reduce_min_sync(kFull, at);
+    if (lane == 0) st->ured[warp] = at;
+    __syncthreads();
+    if (warp == 0) {
+      at = __reduce_min_sync(kFull, st->ured[lane & 15]);
+      if (lane == 0) lead->max_at[rank] = at;
     }
-    return;  // nobody reads or writes another CTA's memory after the barrier above
+    cluster.sync();  // nothing remote is touched after it
+    if (leads && warp == 0) {
+      at = __reduce_min_sync(kFull, lane < ctas ? st->max_at[lane] : 0xffffffffu);
+      if (lane == 0) {
+        const bool none = top == -INFINITY;
+        a.token[r] = none ? -1 : (long long)at;
+        if (a.logprob) a.logprob[r] = none ? NAN : 0.f;
+      }
+    }
+    return;
   }
 
   u64 cut = 0;  // kept: rank keys from the cut on
+  const float slack = fabsf(top) * 1e-6f;  // covers the rounding of max - x
   if (by_count || by_weight) {
     // Fill bins [b0, b1) and bring the cluster's together in the leader's; the
     // first time also add up all weights.
     auto fill = [&](int b0, int b1) {
       u64 sum = 0;
+      // what no bin of these and (the first time) no sum wants goes by fast
+      const float far = b0 == 0 && by_weight ? kSpan : b1 / kBinsPer;
+      const float low = top < INFINITY ? top - far * 1.001f - slack : top;
 #pragma unroll 4
       for (unsigned i = tid; i < s.count; i += kThreads) {
         const float x = s.at(i);
+        if (x < low) continue;
+        const u64 w = by_weight ? weight_of(mass_of(x, top)) : 0;
+        if (b0 == 0) sum += w;
         const int b = bin_of(x, top);
-        const bool in = b >= b0 && b < b1;
-        if (by_count && in) atomicAdd(&st->cbin[b], 1u);
-        if (by_weight && (in || (b0 == 0 && b < kBins))) {
-          const u64 w = weight_of(mass_of(x, top));
-          sum += w;
-          if (in) add_weight(&st->wbin[b], w);
-        }
+        if (b < b0 || b >= b1) continue;
+        if (by_count) atomicAdd(&st->cbin[b], 1u);
+        if (by_weight) add_weight(&st->wbin[b], w);
       }
       if (b0 == 0) {
         const u64 x[2] = {sum, 0};
@@ -445,11 +457,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       if (bin == kBins) continue;
       const unsigned need = which ? 0u : st->verdict.need;
       const u64 goal = which ? st->verdict.goal : 0ull;
-      // gather the bin's rank keys into the leader's list
+      // gather the bin's rank keys into the leader's list; a little beyond its ends
+      // tells the rest off without the bin's arithmetic
+      const float lo = top < INFINITY ? top - (bin + 1) / kBinsPer * 1.001f - slack : top;
+      const float hi = top < INFINITY ? top - bin / kBinsPer * 0.999f + slack : top;
 #pragma unroll 4
       for (unsigned i = tid; i < s.count; i += kThreads) {
         const float x = s.at(i);
-        if (bin_of(x, top) == bin) {
+        if (x >= lo && x <= hi && bin_of(x, top) == bin) {
           const unsigned n = atomicAdd(&lead->listed[which], 1u);
           if (n < kList) lead->list[which][n] = rank_key(x, s.first + i);
         }
@@ -544,8 +559,9 @@ cudaError_t launch_type(const sy_sample_args& a, cudaStream_t st) {
   unsigned slice = (unsigned)((a.vocab + ctas - 1) / ctas);
   slice = (slice + 15) / 16 * 16;
   const bool resident = (int64_t)slice * 4 <= kMaxSlice;
-  const size_t smem = sizeof(State) + (resident ? (size_t)slice * 4 : 0);
-  cudaError_t e = raise_smem_limit(sample_kernel<T>, smem);
+  const size_t smem = kStateBytes + (resident ? (size_t)slice * 4 + 16 : 0);
+  auto* kern = resident ? sample_kernel<T, true> : sample_kernel<T, false>;
+  cudaError_t e = raise_smem_limit(kern, smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a.rows * ctas);
@@ -558,7 +574,7 @@ cudaError_t launch_type(const sy_sample_args& a, cudaStream_t st) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, sample_kernel<T>, a, slice, resident);
+  e = cudaLaunchKernelEx(&cfg, kern, a, slice);
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
