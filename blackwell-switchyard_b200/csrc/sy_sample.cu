@@ -56,7 +56,8 @@ struct Verdict {
 struct State {
   u64 wbin[kBins];       // weight per bin
   unsigned cbin[kBins];  // tokens per bin
-  u64 list[2][kList];    // rank keys gathered for top_k's and top_p's cut
+  u64 list[kList];       // rank keys of this CTA's tokens in the bin that is cut
+  u64 all[kList];        // leader: every CTA's
   u64 sorted[kList];     // also the radix passes' bins
   unsigned listed[2];
   Verdict verdict;
@@ -457,23 +458,37 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       if (bin == kBins) continue;
       const unsigned need = which ? 0u : st->verdict.need;
       const u64 goal = which ? st->verdict.goal : 0ull;
-      // gather the bin's rank keys into the leader's list; a little beyond its ends
-      // tells the rest off without the bin's arithmetic
+      // gather the bin's rank keys; a little beyond its ends tells the rest off
+      // without the bin's arithmetic
       const float lo = top < INFINITY ? top - (bin + 1) / kBinsPer * 1.001f - slack : top;
       const float hi = top < INFINITY ? top - bin / kBinsPer * 0.999f + slack : top;
 #pragma unroll 4
       for (unsigned i = tid; i < s.count; i += kThreads) {
         const float x = s.at(i);
         if (x >= lo && x <= hi && bin_of(x, top) == bin) {
-          const unsigned n = atomicAdd(&lead->listed[which], 1u);
-          if (n < kList) lead->list[which][n] = rank_key(x, s.first + i);
+          const unsigned n = atomicAdd(&st->listed[which], 1u);
+          if (n < kList) st->list[n] = rank_key(x, s.first + i);
         }
       }
       cluster.sync();
-      const unsigned n = lead->listed[which];
+      const unsigned got = lane < ctas ? cluster.map_shared_rank(st, lane)->listed[which] : 0;
+      unsigned upto_got = got;
+#pragma unroll
+      for (int o = 1; o < kMaxCluster; o <<= 1) {
+        const unsigned y = __shfl_up_sync(kFull, upto_got, o);
+        if (lane >= o) upto_got += y;
+      }
+      const unsigned n = __shfl_sync(kFull, upto_got, kMaxCluster - 1);
+      if (leads && n <= kList) {  // a warp or two per CTA bring the lists together
+        const unsigned from = warp % kMaxCluster;
+        const unsigned count = __shfl_sync(kFull, got, from), to = __shfl_sync(kFull, upto_got, from) - count;
+        for (unsigned i = lane + warp / kMaxCluster * 32; i < count; i += kThreads / kMaxCluster)
+          st->all[to + i] = cluster.map_shared_rank(st, from)->list[i];
+        __syncthreads();
+      }
       if (n > kList) radix_cut(st, s, top, bin, need, goal);
       if (leads) {
-        if (n <= kList) rank_list(st, st->list[which], n, need, goal, top);
+        if (n <= kList) rank_list(st, st->all, n, need, goal, top);
         const u64 found = st->found, upto = st->upto;
         __syncthreads();
         if (tid == 0) {
@@ -488,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
           if (st->verdict.p_bin == bin && n <= kList) {  // the same bin: its list is here
             const u64 rest = st->verdict.goal;
             __syncthreads();
-            rank_list(st, st->list[0], n, 0u, rest, top);
+            rank_list(st, st->all, n, 0u, rest, top);
             if (tid == 0) {
               if (st->found > st->verdict.cut) st->verdict.cut = st->found;
               st->verdict.p_bin = kBins;
