@@ -1,8 +1,8 @@
 """Build libswitchyard_b200.so (the C-ABI library) in-tree with nvcc.
 
 Every ``.cu`` file in this directory is compiled for sm_100a only, as
-relocatable device code (the device error word is shared across files; the
-files in ``WHOLE`` have their own), in parallel, then device-linked into one shared library that lands next to the
+relocatable device code (the device error word is shared across files), in
+parallel, then device-linked into one shared library that lands next to the
 Python package that loads it. The library links the *shared* CUDA runtime, so
 in a process that already imported torch it uses torch's runtime and sees the
 same current device.
@@ -38,6 +38,7 @@ FLAGS = [
     "-O3",
     "-std=c++17",
     "-lineinfo",
+    "-rdc=true",
     "-Xcompiler",
     "-fPIC",
     "-Xcompiler",
@@ -45,15 +46,6 @@ FLAGS = [
     "--expt-relaxed-constexpr",
     f"-I{INCLUDE}",
 ]
-
-
-# Files compiled without device linking: ptxas ignores register hand-over between
-# warps (setmaxnreg) in relocatable code. They keep an error word of their own.
-WHOLE = {"sy_attend.cu"}
-
-
-def _mode(src: Path) -> list[str]:
-    return ["-DSY_OWN_ERROR_WORD", "-c"] if src.name in WHOLE else ["-rdc=true", "-dc"]
 
 
 def _nvcc() -> str:
@@ -105,7 +97,7 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False,
     for src in _sources():
         obj = bdir / (src.stem + ".o")
         objs.append(obj)
-        cmds.append([nvcc, *ARCH, *FLAGS, *dflags, "-Xptxas", "-v", *_mode(src), str(src), "-o", str(obj)])
+        cmds.append([nvcc, *ARCH, *FLAGS, *dflags, "-Xptxas", "-v", "-dc", str(src), "-o", str(obj)])
     jobs = jobs or min(len(cmds), os.cpu_count() or 4)
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
         for cmd, rc, log in ex.map(_run, cmds):

@@ -9,7 +9,6 @@
 
 #include "sy_batched.cuh"
 #include "sy_reg.cuh"
-#include "sy_serving.cuh"
 #include "sy_stream.cuh"
 #include "sy_stream_batched.cuh"
 #include "sy_stream_bwd.cuh"
@@ -996,10 +995,7 @@ int sy_device_error(int* code) {
   const unsigned int zero = 0;
   e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof(zero));
   if (e != cudaSuccess) return cuda_error_status(e, "sy_device_error: clear");
-  unsigned int w = 0;
-  e = sy::take_attend_error(&w);
-  if (e != cudaSuccess) return cuda_error_status(e, "sy_device_error: attention's word");
-  *code = (int)(v | w);
+  *code = (int)v;
   return SY_OK;
 }
 

@@ -1081,13 +1081,6 @@ cudaError_t launch_type(const Plan& p, const CUtensorMap& k, const CUtensorMap& 
 
 }  // namespace
 
-cudaError_t take_attend_error(unsigned int* word) {
-  const cudaError_t e = cudaMemcpyFromSymbol(word, g_device_error, sizeof(*word));
-  if (e != cudaSuccess) return e;
-  const unsigned int zero = 0;
-  return cudaMemcpyToSymbol(g_device_error, &zero, sizeof(zero));
-}
-
 int64_t attend_workspace(const sy_attend_args& a, const ServingDev& dev) {
   Plan p;
   return make_plan(a, dev.sms, &p, nullptr);

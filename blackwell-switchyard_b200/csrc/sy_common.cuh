@@ -21,12 +21,7 @@ namespace sy {
 // Device error word. Bit flags; read and cleared by sy_device_error().
 // ---------------------------------------------------------------------------
 enum : unsigned { kDevErrWaitTimeout = 1u, kDevErrBadPlan = 2u, kDevErrBadIndex = 4u };
-#ifdef SY_OWN_ERROR_WORD
-// a file that is compiled on its own (no device linking) has a word of its own
-static __device__ unsigned int g_device_error;
-#else
 extern __device__ unsigned int g_device_error;
-#endif
 
 // A legitimate wait in these kernels lasts microseconds (one HBM round trip
 // plus a few tiles of compute). Two seconds means something is broken.

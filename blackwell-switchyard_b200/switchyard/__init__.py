@@ -3,7 +3,8 @@
 A from-scratch B200-native implementation of the Block AttnRes operator behind
 the Python API of ``sabdulmajid/blackwell-switchyard``'s ``switchyard.triton_op``:
 ``block_attn_res_triton`` (autograd), ``block_attn_res_batched`` (output only),
-``BlockAttnResTriton`` and ``speed_of_light``. The kernels are hand-written CUDA
+``BlockAttnResTriton`` and ``speed_of_light``; and the operators that serve the
+decoder (``append_kv``, ``attend_paged``, ``sample_tokens``). The kernels are hand-written CUDA
 for sm_100a in ``csrc/`` behind the C ABI in ``include/switchyard_b200.h``.
 """
 

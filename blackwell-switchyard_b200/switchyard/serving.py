@@ -85,7 +85,7 @@ def attend_paged(
     no key gets 0 and ``-inf``. What a page holds past its sequence's length
     does not matter, NaN included; keys and values that some query of the call
     sees must be finite. ``head_dim`` is a multiple of 8 up to 128, ``page_size``
-    a multiple of 8. ``scale`` defaults to ``head_dim ** -0.5``.
+    a multiple of 8. ``scale`` is positive and defaults to ``head_dim ** -0.5``.
     """
     out, lse = _sy_torch.attend_paged(q, k_cache, v_cache, page_table, kv_lens, prefix_pages,
                                       prefix_len, scale, return_lse)

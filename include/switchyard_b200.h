@@ -366,7 +366,8 @@ SY_API int64_t sy_attend_workspace(const sy_attend_args* args);
  * A query that sees no key gets out = 0 and lse = -inf. Query head h reads key
  * head h / (q_heads / kv_heads). Own key j is row j % page_size of page
  * page_table[b, j / page_size]; entries past a sequence's length are not read.
- * Rows of a page past the length may hold anything, NaN included. head_dim is
+ * Rows of a page past the length may hold anything, NaN included. scale is
+ * positive and finite. head_dim is
  * a multiple of 8 up to 128 and page_size a multiple of 8; pointers and strides
  * (in bytes) are multiples of 16.
  */

@@ -83,7 +83,7 @@ def test_abi_checks_arguments():
         assert append(**bad) == N.SY_ERR_ARG, bad
 
     good_a = dict(q=16, k_cache=16, v_cache=16, out=16, page_table=16, kv_lens=16, batch=1, q_len=1, q_heads=2,
-                  kv_heads=1, head_dim=64, pages=4, page_size=16, table_width=2, table_row=2)
+                  kv_heads=1, head_dim=64, pages=4, page_size=16, table_width=2, table_row=2, scale=0.125)
 
     def attend(**kw):
         return L.sy_attend(ctypes.byref(Attend(**{**good_a, **kw})), None)
@@ -92,9 +92,12 @@ def test_abi_checks_arguments():
     assert attend(dtype=9) == N.SY_ERR_DTYPE
     for bad in (dict(dtype=N.SY_F32), dict(head_dim=12), dict(head_dim=136), dict(page_size=12)):
         assert attend(**bad) == N.SY_ERR_UNSUPPORTED, bad
+    # query rows further apart than 32 bits of 16 bytes
+    assert attend(q_h=1 << 36) == N.SY_ERR_UNSUPPORTED
+    assert attend(batch=3, q_b=1 << 34) == N.SY_ERR_UNSUPPORTED
     for bad in (dict(q=None), dict(q=8), dict(out=None), dict(kv_lens=None), dict(q_heads=3, kv_heads=2),
                 dict(prefix_len=5), dict(prefix_len=-1), dict(kc_row=4), dict(q_h=3), dict(kc_page=-8),
-                dict(table_width=1 << 28), dict(page_table=None), dict(k_cache=None)):
+                dict(table_width=1 << 28), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(page_table=None), dict(k_cache=None)):
         assert attend(**bad) == N.SY_ERR_ARG, bad
     assert L.sy_attend_workspace(None) == -N.SY_ERR_ARG
 

@@ -356,6 +356,54 @@ def test_attend_indices_outside_are_not_followed(sy):
     assert _native.device_error() == 4 and out.isfinite().all()
 
 
+def test_refusals(sy):
+    args, kw, _, _ = paged(8, [20, 9], 1, 4, 2, 64, 16, 30, torch.bfloat16, junk=0.0)
+    q, kc, vc, table, lens = args
+
+    def no(error, match, *a, **k):
+        with pytest.raises(error, match=match):
+            sy.attend_paged(*a, **{**kw, **k})
+
+    no(ValueError, "dtype", q.half(), kc, vc, table, lens)
+    no(ValueError, "bfloat16 or float16", q.float(), kc.float(), vc.float(), table, lens)
+    no(ValueError, "head_dim", q[..., :60], kc, vc, table, lens)
+    no(ValueError, "multiple of 8", q[..., :60], kc[..., :60], vc[..., :60], table, lens)
+    no(ValueError, "page_size", q, kc[:, :, :12], vc[:, :, :12], table, lens)
+    no(ValueError, "q_heads", q[:, :, :3], kc, vc, table, lens)
+    no(ValueError, "page_table", q, kc, vc, table[:1], lens)
+    no(ValueError, "page_table", q, kc, vc, table.long(), lens)
+    no(ValueError, "kv_lens", q, kc, vc, table, lens.long())
+    no(ValueError, "prefix_pages", *args, prefix_len=33)
+    no(ValueError, "prefix_pages", *args, prefix_pages=None)
+    no(ValueError, "prefix_len", *args, prefix_len=-1)
+    no(ValueError, "last dimension", q, kc.transpose(2, 3).contiguous().transpose(2, 3), vc, table, lens)
+    for scale in (0.0, -1.0, math.nan, math.inf):
+        no(ValueError, "scale", *args, scale=scale)
+    no(ValueError, "CUDA", q, kc, vc, table.cpu(), lens)
+    no(RuntimeError, "no backward", q.clone().requires_grad_(), kc, vc, table, lens)
+
+    x = torch.zeros(2, 2, 64, device="cuda", dtype=torch.bfloat16)
+    slots = torch.zeros(2, device="cuda", dtype=torch.int64)
+    cos, sin = angles(4, 32)
+    pos = slots.int()
+    for bad in (dict(k=x[:, :1]), dict(v=x[:1]), dict(k=x.half()), dict(slots=slots.int()), dict(slots=slots[:1]),
+                dict(q=x[:1]), dict(q=x.float()), dict(positions=pos), dict(positions=pos, cos=cos, sin=sin.half()),
+                dict(positions=pos, cos=cos, sin=sin[:3]), dict(positions=slots, cos=cos, sin=sin),
+                dict(positions=pos, cos=cos.repeat(1, 2), sin=sin.repeat(1, 2))):
+        with pytest.raises(ValueError):
+            sy.append_kv(**{**dict(k=x, v=x, k_cache=kc, v_cache=vc, slots=slots), **bad})
+    with pytest.raises(RuntimeError, match="no backward"):
+        sy.append_kv(x.clone().requires_grad_(), x, kc, vc, slots)
+
+    logits, u = torch.zeros(2, 9, device="cuda"), torch.zeros(2, device="cuda")
+    for bad in (dict(u=u[:1]), dict(u=u.double()), dict(top_k=u), dict(top_p=u[:1]), dict(min_p=u.half()),
+                dict(logits=logits.double()), dict(logits=logits[0])):
+        with pytest.raises(ValueError):
+            sy.sample_tokens(**{**dict(logits=logits, u=u), **bad})
+    with pytest.raises(RuntimeError, match="no backward"):
+        sy.sample_tokens(logits.clone().requires_grad_(), u)
+
+
 # ---------------------------------------------------------------------------
 # sample_tokens
 # ---------------------------------------------------------------------------
