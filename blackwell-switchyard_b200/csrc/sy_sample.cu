@@ -17,7 +17,8 @@
 // The draw then adds the kept weights in index order: CTAs, warps, lanes.
 //
 // The row's bytes are the floor for many rows (256 x 131071 fp32: 20.5 us at the
-// measured copy rate); for one row it is a chain of six to nine cluster barriers.
+// measured copy rate; 244 us, half of the issue slots and about 33 rows in flight);
+// for one row it is a chain of six to nine cluster barriers.
 // A remote shared-memory read costs as much as a barrier, so CTAs push what others
 // need (maxima, sums, the leader's verdicts) ahead of the barrier and read locally.
 #include <cooperative_groups.h>
