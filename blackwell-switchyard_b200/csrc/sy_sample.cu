@@ -287,6 +287,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   const unsigned rank = cluster.block_rank(), ctas = cluster.num_blocks();
   const bool leads = rank == 0;
   State* lead = cluster.map_shared_rank(st, 0);
+  // A CTA's shared memory may only be written from another once it is known to
+  // run: all arrive here and wait before the first push, with the slice's read
+  // in between.
+  cluster.barrier_arrive();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const long long r = blockIdx.x / ctas;
   const unsigned V = (unsigned)a.vocab;
@@ -310,6 +314,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   for (int i = tid; i < kBins; i += kThreads) st->wbin[i] = 0, st->cbin[i] = 0;
   if (tid < 2) st->listed[tid] = 0;
   __syncthreads();
+  cluster.barrier_wait();
   if (warp == 0) {
     top = warp_max(st->fred[lane & 15]);
     if (lane < ctas) cluster.map_shared_rank(st, lane)->max_x[rank] = top;
