@@ -565,14 +565,14 @@ __device__ __forceinline__ void put_rows(const Plan& p, const Cursor& cur, int s
 #pragma unroll 1
   for (int col = 0; col < DP; col += 32) {
     uint32_t o[32];
+    __syncwarp();  // the lanes part where they store; the TMEM load takes the whole warp
     tmem_ld32(o_at + col, o);
     tmem_wait_ld(o);
-    if (!mine) continue;
-    if (!final) {
+    if (mine && !final) {
 #pragma unroll
       for (int k = 0; k < 32; k += 4)
         *reinterpret_cast<uint4*>(dst + (col + k) * 4) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
-    } else {
+    } else if (mine) {
 #pragma unroll
       for (int k = 0; k < 32; k += 8) {
         uint32_t w[4];
@@ -637,6 +637,7 @@ __device__ __forceinline__ void softmax_rows(const Plan& p, char* smem, Bars* ba
             for (int d = 0; d < DP / 64; ++d)
               *reinterpret_cast<uint4*>(v + d * (kTile * 128) + z * 16) = make_uint4(0, 0, 0, 0);
           fence_proxy_async();
+          __syncwarp();  // lanes cleared different numbers of chunks
         }
         if (active) {
           const uint32_t s_at = tmem + lanes + s * kTile + buf * kHalf;
@@ -652,7 +653,7 @@ __device__ __forceinline__ void softmax_rows(const Plan& p, char* smem, Bars* ba
           const bool moves = m == -INFINITY ? top > -INFINITY : top > m + grow<T>() / c;
           if (__any_sync(kFull, moves)) {
             const float keep = !moves ? 1.f : m == -INFINITY ? 0.f : ex2((m - top) * c);
-            if (moves) m = top;
+            m = moves ? top : m;
             l *= keep;
             if (i > 0) {
               // O stands still once the last P V is done: the next needs this step's weights

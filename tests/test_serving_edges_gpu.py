@@ -8,7 +8,15 @@ import math
 import pytest
 import torch
 
-from test_serving_gpu import check_sample, clear_error_word, gen, params, sy  # noqa: F401  (fixtures)
+from test_serving_gpu import (  # noqa: F401  (sy and clear_error_word are fixtures)
+    check_attend,
+    check_sample,
+    clear_error_word,
+    gen,
+    paged,
+    params,
+    sy,
+)
 
 pytestmark = pytest.mark.gpu
 
@@ -40,3 +48,26 @@ def test_sample_many_short_clusters_at_once(sy, vocab):
     for token, lp in got:
         assert torch.equal(token, want.repeat(times))
         assert torch.equal(lp.nan_to_num(1.0), logprob.repeat(times).nan_to_num(1.0))
+
+
+# ---------------------------------------------------------------------------
+# attend_paged
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lens,n,hq,hk,d,page,prefix", [
+    ([130] * 20, 130, 16, 16, 128, 16, 0),  # 320 units: most are finished in one run
+    ([145] * 12, 145, 16, 16, 64, 8, 0),
+    ([131] * 11, 131, 16, 16, 40, 8, 3),
+    ([200, 61, 1], 33, 3, 1, 128, 8, 0),  # 99 rows of a unit; tiles of 72 keys, 61 keys, one key
+    ([97, 98, 99, 100], 1, 21, 1, 128, 24, 131),  # 84 rows over the prefix, 21 over a sequence
+    ([65, 2, 127], 2, 62, 2, 64, 16, 70),  # 62 rows a unit, 186 over the prefix: the second stream has 58
+])
+def test_attend_rows_and_keys_that_leave_lanes_idle(sy, dtype, lens, n, hq, hk, d, page, prefix):
+    """Rows that end inside a warp (its lanes part where O is stored) and keys that end inside a tile (they part where
+    V is cleared): the tensor memory loads that follow take whole warps."""
+    args, kw, lead, own = paged(sum(lens) + n, lens, n, hq, hk, d, page, prefix, dtype)
+    out, lse = sy.attend_paged(*args, **kw, return_lse=True)
+    check_attend(out, lse, args, kw, lead, own)
+    assert torch.equal(sy.attend_paged(*args, **kw), out)
