@@ -123,8 +123,10 @@ def generate(
     ``u`` (fp32 ``[max_new, n_samples]`` in [0, 1)) are the random numbers; without
     it they come from ``generator``. The sampling parameters are
     :func:`~switchyard.sample_tokens`'s. Returns the tokens ``[n_samples, max_new]``
-    and their log-probabilities under the distribution they were drawn from. One
-    host synchronisation at most, when the caller reads the result.
+    and their log-probabilities under the distribution they were drawn from. A
+    sample that meets logits with nothing to draw from (all NaN after an overflow,
+    say) ends there: its tokens are -1 and its log-probabilities NaN from then on.
+    One host synchronisation at most, when the caller reads the result.
     """
     cfg = model.cfg
     weight = model.embed.weight
@@ -170,6 +172,8 @@ def generate(
             break
         slots, positions = cache.own_slots(1), cache.lens + length
         cache.lens += 1
-        h = _step(model, tokens[t][:, None], cache, slots, positions, together)
+        # a sample that has ended goes on with token 0 in the batch; what it draws is dropped below
+        h = _step(model, tokens[t][:, None].clamp(min=0), cache, slots, positions, together)
         logits = model.lm_head(model.final_norm(h[:, -1]))
-    return tokens.t(), logprobs.t()
+    ended = (tokens < 0).cumsum(0) > 0
+    return tokens.masked_fill_(ended, -1).t(), logprobs.masked_fill_(ended, float("nan")).t()
