@@ -142,7 +142,7 @@ def generate(
     if length + max_new > cfg.max_seq_len:
         raise ValueError(f"{length} + {max_new} tokens exceed max_seq_len {cfg.max_seq_len}")
     if u is None:
-        u = torch.rand(max_new, n_samples, generator=generator, device=dev)
+        u = torch.rand(max_new, n_samples, generator=generator, device=dev, dtype=torch.float32)
     elif u.shape != (max_new, n_samples):
         raise ValueError(f"u must be [{max_new}, {n_samples}], got {tuple(u.shape)}")
 
@@ -155,15 +155,13 @@ def generate(
     h = _step(model, prompt[None], cache, cache.prefix_slots(), at, alone)
     logits = model.lm_head(model.final_norm(h[:, -1])).expand(n_samples, -1)
 
-    draw = dict(temperature=torch.full((n_samples,), temperature, device=dev))
-    if top_k is not None:
-        draw["top_k"] = torch.full((n_samples,), top_k, dtype=torch.int32, device=dev)
-    if top_p is not None:
-        draw["top_p"] = torch.full((n_samples,), top_p, device=dev)
-    if min_p is not None:
-        draw["min_p"] = torch.full((n_samples,), min_p, device=dev)
+    def per_sample(x, dtype=torch.float32):
+        return None if x is None else torch.full((n_samples,), x, dtype=dtype, device=dev)
+
+    draw = dict(temperature=per_sample(temperature), top_k=per_sample(top_k, torch.int32),
+                top_p=per_sample(top_p), min_p=per_sample(min_p))
     tokens = torch.empty(max_new, n_samples, dtype=torch.int64, device=dev)
-    logprobs = torch.empty(max_new, n_samples, device=dev)
+    logprobs = torch.empty(max_new, n_samples, dtype=torch.float32, device=dev)
     together = dict(page_table=cache.table, kv_lens=cache.lens, prefix_pages=cache.prefix_pages,
                     prefix_len=length)
     for t in range(max_new):

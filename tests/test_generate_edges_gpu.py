@@ -44,3 +44,36 @@ def test_a_prompt_with_nothing_to_draw_from():
         model.lm_head.weight.fill_(float("nan"))
     tokens, logprobs = generate(model, torch.arange(5, device="cuda"), 3, 4)
     assert (tokens == -1).all() and logprobs.isnan().all()
+
+
+def test_whole_numbers_as_parameters():
+    from switchyard.generate import generate
+
+    model = small()
+    prompt = torch.arange(7, device="cuda")
+    u = torch.rand(3, 5, device="cuda", generator=torch.Generator("cuda").manual_seed(3))
+    want = generate(model, prompt, 5, 3, u=u, temperature=1.0, top_p=1.0, min_p=0.0)
+    got = generate(model, prompt, 5, 3, u=u, temperature=1, top_k=0, top_p=1, min_p=0)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    greedy, _ = generate(model, prompt, 5, 3, u=u, temperature=0)
+    assert torch.equal(greedy, generate(model, prompt, 5, 3, u=u, temperature=0.0)[0])
+
+
+def test_the_default_dtype_does_not_matter():
+    from switchyard.generate import generate
+
+    model = small()
+    prompt = torch.arange(7, device="cuda")
+
+    def draw():
+        g = torch.Generator("cuda").manual_seed(4)
+        return generate(model, prompt, 5, 3, temperature=0.8, top_p=0.9, min_p=0.01, generator=g)
+
+    want = draw()
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(torch.bfloat16)
+    try:
+        got = draw()
+    finally:
+        torch.set_default_dtype(before)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and got[1].dtype == torch.float32
