@@ -34,6 +34,8 @@ class PagedCache:
                  own_len: int, dtype: torch.dtype, device, page_size: int = 64) -> None:
         if batch < 1 or prefix_len < 0 or own_len < 0:
             raise ValueError("batch must be positive, prefix_len and own_len not negative")
+        if page_size < 1 or page_size % 8:
+            raise ValueError(f"page_size must be a positive multiple of 8, got {page_size}")
         ahead, own = -(-prefix_len // page_size), -(-own_len // page_size)
         self.page_size, self.prefix_len = page_size, prefix_len
         self.kv = torch.empty(layers, 2, ahead + batch * own, heads, page_size, head_dim,

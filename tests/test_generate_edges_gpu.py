@@ -77,3 +77,11 @@ def test_the_default_dtype_does_not_matter():
     finally:
         torch.set_default_dtype(before)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and got[1].dtype == torch.float32
+
+
+@pytest.mark.parametrize("page_size", [0, -8, 12])
+def test_page_sizes_that_are_refused(page_size):
+    from switchyard.generate import generate
+
+    with pytest.raises(ValueError, match="page_size"):
+        generate(small(), torch.arange(7, device="cuda"), 2, 3, page_size=page_size)
