@@ -85,13 +85,19 @@ __global__ void __launch_bounds__(256, 6)
   const bool bad_pos = h && (pos < 0 || pos >= a.rope_len);
   const bool bad_slot = slot >= a.pages * a.page_size;
   if (bad_pos || bad_slot) {
-    // not followed: the token's cache rows stay as they were, its q is zero
+    // not followed: the token's cache rows stay as they were, and its q is zero if
+    // the position was outside (rotated as ever if only the slot was)
     if (threadIdx.x == 0) record_device_error(kDevErrBadIndex);
     slot = -1;
   }
-  const float* cs = a.cos + (bad_pos ? 0 : pos) * a.rope_row;
-  const float* sn = a.sin + (bad_pos ? 0 : pos) * a.rope_row;
   const int nq = (int)a.q_heads, nk = (int)a.kv_heads;
+  if (bad_pos) {
+    T* q = static_cast<T*>(a.q_out) + t * nq * (long long)d;
+    for (int i = threadIdx.x; i < nq * d; i += blockDim.x) q[i] = Dt<T>::from_f(0.f);
+    return;
+  }
+  const float* cs = a.cos + pos * a.rope_row;
+  const float* sn = a.sin + pos * a.rope_row;
   long long page = 0, row = 0;
   if (slot >> 32) {
     if (slot > 0) page = slot / a.page_size, row = slot - page * a.page_size;
@@ -127,7 +133,7 @@ __global__ void __launch_bounds__(256, 6)
       load_angles<VEC>(sn + c * VEC, angles16, si);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        const float u = bad_pos ? 0.f : Dt<T>::to_f(x1.e[i]), w = bad_pos ? 0.f : Dt<T>::to_f(x2.e[i]);
+        const float u = Dt<T>::to_f(x1.e[i]), w = Dt<T>::to_f(x2.e[i]);
         x1.e[i] = Dt<T>::from_f(__fsub_rn(__fmul_rn(u, co[i]), __fmul_rn(w, si[i])));
         x2.e[i] = Dt<T>::from_f(__fadd_rn(__fmul_rn(w, co[i]), __fmul_rn(u, si[i])));
       }

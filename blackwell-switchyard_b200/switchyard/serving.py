@@ -51,7 +51,9 @@ def append_kv(
     ``positions`` (int32 ``[tokens]``) are rows of ``cos`` and ``sin`` (fp32
     ``[length, r]``, :func:`switchyard.decoder.rope_tables`): columns ``i`` and
     ``i + r`` of a head, ``i < r``, turn against each other, the columns from
-    ``2 r`` on are kept. Without the three nothing is rotated.
+    ``2 r`` on are kept. Without the three nothing is rotated. A token whose
+    slot or position lies outside writes nothing to the caches; its rotated
+    ``q`` is zero if the position does, and as ever if only the slot does.
     """
     return _sy_torch.append_kv(k, v, k_cache, v_cache, slots, q, positions, cos, sin)
 

@@ -331,7 +331,9 @@ typedef struct sy_append_kv_args {
  *   y[i] = x[i] for i >= 2h
  * in fp32 with one rounding. q_out = rotated q; the rotated k and the v of
  * every token with slot >= 0 are written to their rows of the caches. Two live
- * tokens with one slot race. One launch.
+ * tokens with one slot race. One launch. A token whose slot or position is
+ * outside writes no cache row; its q_out is zero if the position is outside, and
+ * rotated as ever if only the slot is.
  */
 SY_API int sy_append_kv(const sy_append_kv_args* args, sy_stream_t stream);
 

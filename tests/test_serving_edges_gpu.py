@@ -9,10 +9,12 @@ import pytest
 import torch
 
 from test_serving_gpu import (  # noqa: F401  (sy and clear_error_word are fixtures)
+    angles,
     check_attend,
     check_sample,
     clear_error_word,
     gen,
+    near_turned,
     paged,
     params,
     sy,
@@ -71,3 +73,29 @@ def test_attend_rows_and_keys_that_leave_lanes_idle(sy, dtype, lens, n, hq, hk, 
     out, lse = sy.attend_paged(*args, **kw, return_lse=True)
     check_attend(out, lse, args, kw, lead, own)
     assert torch.equal(sy.attend_paged(*args, **kw), out)
+
+
+# ---------------------------------------------------------------------------
+# append_kv
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_append_what_q_holds_for_indices_outside(sy, dtype):
+    """Partial rotation: q is zero in all its columns where the position lies outside, and rotated as ever where only
+    the slot does. The cache rows of both tokens stay as they were."""
+    from switchyard import _native
+
+    kc, vc = (torch.full((2, 1, 8, 40), 7.0, device="cuda", dtype=dtype) for _ in range(2))
+    cos, sin = angles(4, 8)
+    x = torch.randn(4, 1, 40, generator=gen(1), device="cuda").to(dtype)
+    pos = torch.tensor([0, 4, -1, 3], device="cuda", dtype=torch.int32)
+    q = sy.append_kv(x, x, kc, vc, torch.tensor([3, 1, 2, 16], device="cuda"), q=x, positions=pos, cos=cos, sin=sin)
+    assert _native.device_error() == 4
+    assert not q[1:3].any()
+    for t in (0, 3):
+        near_turned(q[t:t + 1], x[t:t + 1], cos[pos[t:t + 1].long()], sin[pos[t:t + 1].long()])
+    kept = torch.ones(2, 8, dtype=torch.bool, device="cuda")
+    kept[0, 3] = False
+    assert (kc[:, 0][kept] == 7).all() and (vc[:, 0][kept] == 7).all()
+    assert torch.equal(vc[0, :, 3], x[0])
