@@ -62,16 +62,18 @@ int check_attend(const sy_attend_args* a, bool pointers) {
   if ((a->table_width > 0 || a->prefix_len > 0) && a->pages > 0 && (!a->k_cache || !a->v_cache))
     return SY_ERR_ARG;
   if (!al16(a->q) || !al16(a->k_cache) || !al16(a->v_cache) || !al16(a->out)) return SY_ERR_ARG;
-  const int64_t strides[] = {a->q_b,     a->q_t,    a->q_h,     a->kc_page, a->kc_head,
-                             a->kc_row, a->vc_page, a->vc_head, a->vc_row};
-  for (int64_t s : strides)
-    if (s < 0 || s % 8 != 0 || s > (int64_t(1) << 38)) return SY_ERR_ARG;
+  // {length, stride} of each axis; that of one element may carry any stride
+  const int64_t axes[][2] = {{a->batch, a->q_b},         {a->q_len, a->q_t},        {a->q_heads, a->q_h},
+                             {a->pages, a->kc_page},     {a->kv_heads, a->kc_head}, {a->page_size, a->kc_row},
+                             {a->pages, a->vc_page},     {a->kv_heads, a->vc_head}, {a->page_size, a->vc_row}};
+  for (const auto& x : axes)
+    if (x[0] > 1 && (x[1] < 0 || x[1] % 8 != 0 || x[1] > (int64_t(1) << 38))) return SY_ERR_ARG;
   // the kernel counts the start of a query row in 32 bits, in units of 16 bytes
   int64_t reach = 0;
-  const int64_t steps[3][2] = {{a->batch, a->q_b}, {a->q_len, a->q_t}, {a->q_heads, a->q_h}};
-  for (const auto& s : steps) {
-    if (s[0] > 1 && s[1] > (int64_t(1) << 35) / (s[0] - 1)) return SY_ERR_UNSUPPORTED;
-    reach += (s[0] - 1) * s[1];
+  for (int i = 0; i < 3; ++i) {
+    const int64_t more = axes[i][0] - 1, step = axes[i][1];
+    if (more > 0 && step > (int64_t(1) << 35) / more) return SY_ERR_UNSUPPORTED;
+    reach += more > 0 ? more * step : 0;
   }
   if (reach >= int64_t(1) << 35) return SY_ERR_UNSUPPORTED;
   return SY_OK;

@@ -201,6 +201,14 @@ at::Tensor last_contiguous(const at::Tensor& t) {
   return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous();
 }
 
+// Rows of 16-bit elements that all start at multiples of 16 bytes (an axis of one
+// element may carry any stride).
+bool rows_aligned(const at::Tensor& t) {
+  for (int64_t i = 0; i + 1 < t.dim(); ++i)
+    if (t.size(i) > 1 && t.stride(i) % 8) return false;
+  return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+}
+
 // Rotated q (undefined without q); the caches are written.
 OptTensor append_kv(const at::Tensor& k_in, const at::Tensor& v_in, const at::Tensor& kc,
                     const at::Tensor& vc, const at::Tensor& slots_in, const OptTensor& q_in,
@@ -290,9 +298,7 @@ std::tuple<at::Tensor, OptTensor> attend_paged(const at::Tensor& q_in, const at:
   TORCH_CHECK_VALUE(d % 8 == 0 && d <= 128, "head_dim must be a multiple of 8 up to 128, got ", d);
   TORCH_CHECK_VALUE(page % 8 == 0, "page_size must be a multiple of 8, got ", page);
   for (const at::Tensor* c : {&kc, &vc})
-    for (int64_t i = 0; i < 3; ++i)
-      TORCH_CHECK_VALUE(c->stride(i) % 8 == 0 && reinterpret_cast<uintptr_t>(c->data_ptr()) % 16 == 0,
-                        "the caches' rows must start at multiples of 16 bytes");
+    TORCH_CHECK_VALUE(rows_aligned(*c), "the caches' rows must start at multiples of 16 bytes");
   TORCH_CHECK_VALUE(table_in.dim() == 2 && table_in.size(0) == b, "page_table must be [", b,
                     ", pages a sequence], got ", shape_of(table_in));
   same_device(table_in, kc, "page_table");
@@ -314,8 +320,7 @@ std::tuple<at::Tensor, OptTensor> attend_paged(const at::Tensor& q_in, const at:
   }
   const c10::cuda::CUDAGuard guard(kc.device());
   at::Tensor q = q_in;
-  if (q.numel() && (q.stride(3) != 1 || q.stride(0) % 8 || q.stride(1) % 8 || q.stride(2) % 8 ||
-                    reinterpret_cast<uintptr_t>(q.data_ptr()) % 16))
+  if (q.numel() && (q.stride(3) != 1 || !rows_aligned(q)))
     q = q.clone(at::MemoryFormat::Contiguous);
   at::Tensor out = at::empty({b, n, hq, d}, q.options());
   OptTensor lse;

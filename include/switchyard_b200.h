@@ -371,7 +371,8 @@ SY_API int64_t sy_attend_workspace(const sy_attend_args* args);
  * Rows of a page past the length may hold anything, NaN included. scale is
  * positive and finite. head_dim is
  * a multiple of 8 up to 128 and page_size a multiple of 8; pointers and strides
- * (in bytes) are multiples of 16.
+ * (in bytes) are multiples of 16 (the stride of an axis of one element is not
+ * read).
  */
 SY_API int sy_attend(const sy_attend_args* args, sy_stream_t stream);
 

@@ -99,3 +99,19 @@ def test_append_what_q_holds_for_indices_outside(sy, dtype):
     kept[0, 3] = False
     assert (kc[:, 0][kept] == 7).all() and (vc[:, 0][kept] == 7).all()
     assert torch.equal(vc[0, :, 3], x[0])
+
+
+def test_attend_axes_of_one_element_may_have_any_stride(sy):
+    """A cache of one page, and one of one key head, whose strides along those axes are no multiples of 16 bytes."""
+    for lens, hk in (([13], 2), ([40, 5], 1)):
+        args, kw, lead, own = paged(9, lens, 1, 4, hk, 64, 64, 0, torch.bfloat16)
+        q, kc, vc, table, n = args
+        if hk == 2:  # one page alone
+            page = int(table[0, 0])
+            kc, vc, table = kc[page:page + 1], vc[page:page + 1], torch.zeros_like(table)
+        want = sy.attend_paged(q, kc, vc, table, n)
+        strides = [(s if m > 1 else 13) for s, m in zip(kc.stride(), kc.shape)]
+        odd = [torch.as_strided(c, c.shape, strides, c.storage_offset()) for c in (kc, vc)]
+        assert torch.equal(sy.attend_paged(q, *odd, table, n), want)
+        thin = [torch.as_strided(x, x.shape, [3 if m == 1 else s for s, m in zip(x.stride(), x.shape)]) for x in (q,)]
+        assert torch.equal(sy.attend_paged(*thin, kc, vc, table, n), want)
