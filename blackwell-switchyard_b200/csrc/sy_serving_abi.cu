@@ -54,7 +54,8 @@ int check_attend(const sy_attend_args* a, bool pointers) {
     return SY_ERR_ARG;
   if (a->table_width * a->page_size >= kMaxCount) return SY_ERR_ARG;
   if (a->batch * a->q_len >= kMaxCount / a->q_heads) return SY_ERR_ARG;
-  if (!(a->scale > 0.f) || a->scale > 3.0e38f) return SY_ERR_ARG;
+  // the kernels multiply by scale * log2(e), which has to be finite too
+  if (!(a->scale > 0.f) || a->scale > 2.35e38f) return SY_ERR_ARG;
   if (!pointers || a->batch == 0 || a->q_len == 0) return SY_OK;
   if (!a->q || !a->out || !a->kv_lens) return SY_ERR_ARG;
   if (a->prefix_len > 0 && !a->prefix_pages) return SY_ERR_ARG;

@@ -305,8 +305,9 @@ std::tuple<at::Tensor, OptTensor> attend_paged(const at::Tensor& q_in, const at:
   need_dtype(table_in, at::kInt, "page_table");
   const at::Tensor lens = index_vector(lens_in, b, at::kInt, kc, "kv_lens");
   const at::Tensor table = last_contiguous(table_in);
-  TORCH_CHECK_VALUE(!scale || (*scale > 0.0 && std::isfinite(*scale)),
-                    "scale must be positive and finite, got ", scale.value_or(0.0));
+  TORCH_CHECK_VALUE(!scale || (*scale <= 2.35e38 && static_cast<float>(*scale) > 0.f),
+                    "scale must be positive and finite, in 32 bits and times log2(e), got ",
+                    scale.value_or(0.0));
   TORCH_CHECK_VALUE(prefix_len >= 0, "prefix_len must not be negative, got ", prefix_len);
   at::Tensor prefix;
   if (prefix_len > 0) {

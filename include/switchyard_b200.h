@@ -369,7 +369,7 @@ SY_API int64_t sy_attend_workspace(const sy_attend_args* args);
  * head h / (q_heads / kv_heads). Own key j is row j % page_size of page
  * page_table[b, j / page_size]; entries past a sequence's length are not read.
  * Rows of a page past the length may hold anything, NaN included. scale is
- * positive and finite. head_dim is
+ * positive and at most 2.35e38 (the kernel multiplies it by log2(e)). head_dim is
  * a multiple of 8 up to 128 and page_size a multiple of 8; pointers and strides
  * (in bytes) are multiples of 16 (the stride of an axis of one element is not
  * read).

@@ -18,3 +18,12 @@ def test_strides_of_the_abi():
         for stride in (4, -8, (1 << 38) + 8):
             args = Attend(**{**good, axis: stride})
             assert N.lib.sy_attend(ctypes.byref(args), None) == N.SY_ERR_ARG, (axis, stride)
+
+
+def test_scale_times_log2_e_must_be_finite():
+    """The kernels take their exponentials to base 2: a scale that overflows there gave NaN."""
+    from switchyard import _native as N
+
+    nothing = dict(q_len=1, q_heads=2, kv_heads=1, head_dim=64, pages=4, page_size=16)
+    for scale, want in ((2.3e38, N.SY_OK), (2.4e38, N.SY_ERR_ARG), (2.9e38, N.SY_ERR_ARG)):
+        assert N.lib.sy_attend(ctypes.byref(Attend(batch=0, scale=scale, **nothing)), None) == want, scale

@@ -115,3 +115,12 @@ def test_attend_axes_of_one_element_may_have_any_stride(sy):
         assert torch.equal(sy.attend_paged(q, *odd, table, n), want)
         thin = [torch.as_strided(x, x.shape, [3 if m == 1 else s for s, m in zip(x.stride(), x.shape)]) for x in (q,)]
         assert torch.equal(sy.attend_paged(*thin, kc, vc, table, n), want)
+
+
+def test_attend_scale_that_overflows_is_refused(sy):
+    args, kw, _, _ = paged(10, [20], 1, 2, 2, 64, 16, 0, torch.bfloat16)
+    for scale in (2.4e38, 1e39, 1e-46):  # the last is zero in 32 bits
+        with pytest.raises(ValueError, match="scale"):
+            sy.attend_paged(*args, scale=scale)
+    out = sy.attend_paged(args[0].zero_(), *args[1:], scale=2.3e38)
+    assert out.isfinite().all()
