@@ -397,11 +397,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     // The leader's threads have four bins each; tokens and weight before them.
     constexpr int kEach = kBins / kThreads;
     u64 before[2], z = 0;
+    auto p_of_z = [&]() -> u64 {
+      const double g = ceil((double)fmaxf(p, 0.f) * (double)z);
+      return g < 1.0 ? 1ull : min((u64)g, z);
+    };
     // The bin where the weight reaches p of z (the last one allowed at the latest).
     auto find_weight = [&](int last) {
-      const double g = ceil((double)fmaxf(p, 0.f) * (double)z);
-      u64 goal = g < 1.0 ? 1ull : (u64)g;
-      if (goal > z) goal = z;
+      const u64 goal = p_of_z();
       u64 weight = before[1];
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
@@ -427,8 +429,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       z = lane < ctas ? st->sums[lane] : 0;
       z = warp_sum64(z);
       // enough, if k tokens were counted, or the weight that p asks for at most
-      const double g = ceil((double)fmaxf(p, 0.f) * (double)z);
-      const bool enough = all_filled || (by_count ? sums[0] >= (u64)k : (double)sums[1] >= g);
+      // (in whole numbers: a sum beyond 2^53 rounds up to a goal that it does not reach)
+      const bool enough = all_filled || (by_count ? sums[0] >= (u64)k : sums[1] >= p_of_z());
       if (tid == 0) {
         st->verdict.enough = enough;
         st->verdict.k_bin = st->verdict.p_bin = kBins;

@@ -52,6 +52,39 @@ def test_sample_many_short_clusters_at_once(sy, vocab):
         assert torch.equal(lp.nan_to_num(1.0), logprob.repeat(times).nan_to_num(1.0))
 
 
+def test_sample_top_p_cut_between_two_doubles(sy):
+    """Sums of weights beyond 2^53 and a cut right behind what the bins next to the maximum hold: S = 2^60 + W, a
+    number that no double is, and a goal of S + 64, the double that S rounds to. One more token than those bins' is
+    kept, the highest of the rest."""
+    d = torch.arange(6.94, 7.1, 2.0**-21, dtype=torch.float64, device="cuda").float()
+    w = ((-d).exp().double() * 2.0**40).round().long()
+    near = int((w % 256 == 192).nonzero()[0])  # 2^60 + w is 64 below a multiple of 256
+    s = 2**60 + int(w[near])
+    goal = s + 64
+    assert int(float(s)) == goal and goal % 256 == 0
+    p = 1.0 - 2.0**-24
+    # lower weights so that p of the total is the goal
+    table = torch.linspace(7.2, 27.0, 200_000, dtype=torch.float64, device="cuda").float()
+    weights = ((-table).exp().double() * 2.0**40).round().long().cpu().numpy()
+    total, rest, at = math.ceil(goal / p), [], 0
+    left = total - s
+    table = table.cpu().numpy()
+    while left > 0:
+        at += int((weights[at:] <= left).argmax())
+        if weights[at] > left:
+            break
+        rest.append(float(table[at]))
+        left -= int(weights[at])
+    total -= left
+    assert math.ceil(p * float(total)) == goal, "the inputs are as described"
+    x = torch.cat([-torch.tensor(rest[::-1], device="cuda"), torch.zeros(2**20, device="cuda"), -d[near:near + 1]])
+    ones = torch.ones(2, device="cuda")
+    u = torch.tensor([0.0, 1.0 - 2.0**-24], device="cuda")
+    token = sy.sample_tokens(x.expand(2, -1), u, top_p=p * ones)
+    assert int(token[0]) == rest[::-1].index(rest[0]), "of the rest only the highest, at its lowest index, is kept"
+    check_sample(sy, x.expand(2, -1), u, ones, 0 * ones.int(), p * ones, 0 * ones)
+
+
 # ---------------------------------------------------------------------------
 # attend_paged
 # ---------------------------------------------------------------------------
