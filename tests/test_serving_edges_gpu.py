@@ -85,6 +85,25 @@ def test_sample_top_p_cut_between_two_doubles(sy):
     check_sample(sy, x.expand(2, -1), u, ones, 0 * ones.int(), p * ones, 0 * ones)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [262145, 700_001, 1 << 22])
+def test_sample_slices_beyond_shared_memory(sy, dtype, vocab):
+    """Slices that do not fit in shared memory are read again from global memory: random rows, one of equal logits and
+    one of few values (more ties in a bin than its list holds)."""
+    x = 3 * torch.randn(5, vocab, generator=gen(vocab), device="cuda")
+    x[0] = 1.0
+    x[1] = x[1].round()
+    x[2] = torch.where(x[2] > 2, x[2], -math.inf)
+    x = x.to(dtype)
+    u = torch.rand(5, generator=gen(1), device="cuda")
+    one = torch.ones(5, device="cuda")
+    zero = torch.zeros_like(one)
+    check_sample(sy, x, u, 0.7 * one, 60 + zero.int(), 0.8 * one, zero)
+    check_sample(sy, x, u, one, zero.int(), 0.9 * one, 0.01 * one)
+    check_sample(sy, x, u, one, zero.int(), one, zero)
+    check_sample(sy, x, u, zero, zero.int(), one, zero)
+
+
 # ---------------------------------------------------------------------------
 # attend_paged
 # ---------------------------------------------------------------------------
@@ -103,6 +122,22 @@ def test_attend_rows_and_keys_that_leave_lanes_idle(sy, dtype, lens, n, hq, hk, 
     """Rows that end inside a warp (its lanes part where O is stored) and keys that end inside a tile (they part where
     V is cleared): the tensor memory loads that follow take whole warps."""
     args, kw, lead, own = paged(sum(lens) + n, lens, n, hq, hk, d, page, prefix, dtype)
+    out, lse = sy.attend_paged(*args, **kw, return_lse=True)
+    check_attend(out, lse, args, kw, lead, own)
+    assert torch.equal(sy.attend_paged(*args, **kw), out)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lens,n,hq,hk,d,page,prefix", [
+    ([7] * 75, 1, 32, 8, 128, 16, 300),  # 300 rows over the prefix: two row tiles, the second with 44
+    ([1, 50, 9] * 43, 1, 32, 8, 64, 8, 129),  # 516 rows: a third tile of four rows
+    ([30] * 5, 30, 8, 2, 128, 64, 200),  # 120 rows a sequence, 600 over the prefix
+    ([3] * 400, 1, 4, 4, 64, 8, 20),  # two sequences a thread in the scan over the lengths
+    ([0, 1, 0, 130, 5] * 160, 1, 8, 2, 128, 16, 0),  # 800 sequences, some of them empty
+    ([5] * 389, 5, 6, 2, 80, 8, 0),
+])
+def test_attend_many_sequences(sy, dtype, lens, n, hq, hk, d, page, prefix):
+    args, kw, lead, own = paged(len(lens), lens, n, hq, hk, d, page, prefix, dtype)
     out, lse = sy.attend_paged(*args, **kw, return_lse=True)
     check_attend(out, lse, args, kw, lead, own)
     assert torch.equal(sy.attend_paged(*args, **kw), out)
