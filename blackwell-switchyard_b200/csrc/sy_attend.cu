@@ -296,7 +296,7 @@ __device__ __forceinline__ void load_tiles(const Plan& p, const CUtensorMap* kma
           row = key - at * ps;
           if (page < 0 || page >= p.a.pages) {
             record_device_error(kDevErrBadIndex);
-            page = (int)p.a.pages;  // past the tensor: the copy fills zeros
+            page = (int)p.a.pages;  // past the tensor: the copy fills zeros, which count as keys
           }
         }
 #pragma unroll 1

@@ -10,8 +10,8 @@ strides whose last one is 1, e.g. one layer of ``[layers, 2, pages, ...]``).
 run on the caller's current stream, allocate with torch's caching allocator and
 do not synchronise; lengths, page numbers, slots and positions are read on the
 device, so a captured CUDA graph replays with new ones. An index outside its
-buffer is not followed: the kernel skips it and sets bit 4 of
-``_native.device_error()``. None of the three has a backward.
+buffer is not followed and sets bit 4 of ``_native.device_error()``; each
+function says what stands in for it. None of the three has a backward.
 
 * :func:`append_kv` -- rotate the new queries and keys, write the new keys and
   values to their slots (``sy_append_kv``);
@@ -86,7 +86,9 @@ def attend_paged(
     q_len, q_heads]`` logarithm of the softmax's denominator. A query that sees
     no key gets 0 and ``-inf``. What a page holds past its sequence's length
     does not matter, NaN included; keys and values that some query of the call
-    sees must be finite. ``head_dim`` is a multiple of 8 up to 128, ``page_size``
+    sees must be finite. A page outside the cache counts as keys and values of
+    zero, a length outside ``[0, width * page_size]`` as the nearer end; both
+    set the error bit, and the result is not to be used. ``head_dim`` is a multiple of 8 up to 128, ``page_size``
     a multiple of 8. ``scale`` is positive and defaults to ``head_dim ** -0.5``.
     """
     out, lse = _sy_torch.attend_paged(q, k_cache, v_cache, page_table, kv_lens, prefix_pages,

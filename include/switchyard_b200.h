@@ -304,7 +304,10 @@ SY_API int64_t sy_dw_exchange_bytes(int64_t L, int world);
  * row s % page_size of page s / page_size. Indices that come from device
  * memory (slots, positions, page numbers, lengths) are checked by the kernels:
  * one outside its buffer is not followed and sets bit 4 of the device error
- * word (sy_device_error).
+ * word (sy_device_error). What stands in for it: sy_append_kv writes no cache
+ * row of that token; sy_attend takes the keys and values of a page outside the
+ * cache for zeros (they count in the softmax, with score 0) and a length outside
+ * [0, table_width * page_size] for the nearer end.
  */
 typedef struct sy_append_kv_args {
   const void* q; /* [tokens, q_heads, head_dim] or NULL (q_heads 0) */

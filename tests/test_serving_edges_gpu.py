@@ -192,3 +192,29 @@ def test_attend_scale_that_overflows_is_refused(sy):
             sy.attend_paged(*args, scale=scale)
     out = sy.attend_paged(args[0].zero_(), *args[1:], scale=2.3e38)
     assert out.isfinite().all()
+
+
+def test_attend_what_stands_in_for_indices_outside(sy):
+    """A page outside the cache reads as zero keys and values, which count; a length outside is cut to the table."""
+    from switchyard import _native
+
+    args, kw, lead, own = paged(7, [40, 48], 1, 4, 4, 64, 16, 37, torch.bfloat16)
+    q, kc, vc, table, lens = args
+    for page in (kc.shape[0], -1, 2**31 - 1):
+        bad = table.clone()
+        bad[0, 1] = page
+        out, lse = sy.attend_paged(q, kc, vc, bad, lens, **kw, return_lse=True)
+        assert _native.device_error() == 4
+        zeroed = [[side[0].clone(), side[1]] for side in own]
+        for side in zeroed:
+            side[0][:, 16:32] = 0
+        check_attend(out, lse, args, kw, lead, zeroed)
+    # a table of exactly three pages: sequence 1 fills it
+    whole = table[:, :3].contiguous()
+    want = sy.attend_paged(q, kc, vc, whole, lens, **kw)
+    far = torch.stack([lens[0], torch.full_like(lens[0], 2**31 - 1)])
+    assert torch.equal(sy.attend_paged(q, kc, vc, whole, far, **kw), want)
+    assert _native.device_error() == 4
+    out, lse = sy.attend_paged(q, kc, vc, table, torch.stack([lens[0], -lens[1]]), **kw, return_lse=True)
+    assert _native.device_error() == 4
+    check_attend(out, lse, args, kw, lead, [[side[0], side[1][:, :0]] for side in own])
