@@ -970,7 +970,6 @@ __global__ void __launch_bounds__(32 * kJoinWarps, 4) join_kernel(const __grid_c
 }
 
 // No page anywhere: every row is empty.
-template <typename T>
 __global__ void __launch_bounds__(256) no_keys_kernel(const sy_attend_args a) {
   const long long i = blockIdx.x * 256ll + threadIdx.x;
   const long long rows = a.batch * a.q_len * a.q_heads;
@@ -1097,7 +1096,7 @@ int64_t attend_workspace(const sy_attend_args& a, const ServingDev& dev) {
 cudaError_t launch_attend(const sy_attend_args& a, const ServingDev& dev, cudaStream_t st) {
   if (a.pages == 0 || (a.table_width == 0 && a.prefix_len == 0)) {
     const int64_t n = a.batch * a.q_len * a.q_heads * (a.head_dim / 8);
-    return launch_smem(no_keys_kernel<__half>, dim3((unsigned)((n + 255) / 256)), 256, 0, st, a);
+    return launch_smem(no_keys_kernel, dim3((unsigned)((n + 255) / 256)), 256, 0, st, a);
   }
   Plan p;
   make_plan(a, dev.sms, &p, static_cast<char*>(a.workspace));

@@ -603,9 +603,7 @@ cudaError_t launch_type(const sy_sample_args& a, cudaStream_t st) {
 
 }  // namespace
 
-int64_t sample_workspace(const sy_sample_args&, const ServingDev&) { return 0; }
-
-cudaError_t launch_sample(const sy_sample_args& a, const ServingDev&, cudaStream_t st) {
+cudaError_t launch_sample(const sy_sample_args& a, cudaStream_t st) {
   switch (a.dtype) {
     case SY_BF16:
       return launch_type<__nv_bfloat16>(a, st);

@@ -20,7 +20,6 @@ cudaError_t launch_append(const sy_append_kv_args& a, cudaStream_t st);
 int64_t attend_workspace(const sy_attend_args& a, const ServingDev& dev);
 cudaError_t launch_attend(const sy_attend_args& a, const ServingDev& dev, cudaStream_t st);
 
-int64_t sample_workspace(const sy_sample_args& a, const ServingDev& dev);
-cudaError_t launch_sample(const sy_sample_args& a, const ServingDev& dev, cudaStream_t st);
+cudaError_t launch_sample(const sy_sample_args& a, cudaStream_t st);
 
 }  // namespace sy

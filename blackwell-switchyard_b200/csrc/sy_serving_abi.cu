@@ -130,25 +130,14 @@ int sy_attend(const sy_attend_args* args, sy_stream_t stream) {
 
 int64_t sy_sample_workspace(const sy_sample_args* args) {
   const int st = sy::check_sample(args, false);
-  if (st != SY_OK) return -st;
-  if (args->rows == 0) return 0;
-  sy::ServingDev dev;
-  const cudaError_t e = sy::serving_dev(&dev);
-  if (e != cudaSuccess) return -sy::cuda_error_status(e, "sy_sample_workspace");
-  return sy::sample_workspace(*args, dev);
+  return st == SY_OK ? 0 : -st;
 }
 
 int sy_sample(const sy_sample_args* args, sy_stream_t stream) {
   const int st = sy::check_sample(args, true);
   if (st != SY_OK || args->rows == 0) return st;
-  sy::ServingDev dev;
-  const cudaError_t e = sy::serving_dev(&dev);
-  if (e != cudaSuccess) return sy::cuda_error_status(e, "sy_sample");
-  if (args->workspace_bytes < sy::sample_workspace(*args, dev) ||
-      (args->workspace_bytes > 0 && (!args->workspace || !sy::al16(args->workspace))))
-    return SY_ERR_ARG;
-  return sy::cuda_error_status(sy::launch_sample(*args, dev, static_cast<cudaStream_t>(stream)),
-                       "sy_sample");
+  return sy::cuda_error_status(sy::launch_sample(*args, static_cast<cudaStream_t>(stream)),
+                               "sy_sample");
 }
 
 }  // extern "C"

@@ -387,14 +387,6 @@ std::tuple<at::Tensor, OptTensor> sample_tokens(const at::Tensor& logits_in, con
   a.token = token.data_ptr<int64_t>();
   a.logprob = want_logprob ? logprob->data_ptr<float>() : nullptr;
   a.rows = rows, a.vocab = vocab, a.logits_row = rows > 1 ? logits.stride(0) : vocab;
-  const int64_t bytes = sy_sample_workspace(&a);
-  TORCH_CHECK(bytes >= 0, "switchyard: sy_sample_workspace failed (status ", -bytes, "): ",
-              sy_status_string(static_cast<int>(-bytes)));
-  at::Tensor ws;
-  if (bytes > 0) {
-    ws = at::empty({bytes}, logits.options().dtype(at::kByte));
-    a.workspace = ws.data_ptr(), a.workspace_bytes = bytes;
-  }
   check(sy_sample(&a, stream_of(logits)), "sy_sample");
   return {token, logprob};
 }

@@ -388,13 +388,14 @@ typedef struct sy_sample_args {
   const float* min_p;       /* [rows] or NULL (off); <= 0 is off */
   int64_t* token;           /* [rows] */
   float* logprob;           /* [rows] or NULL */
-  void* workspace;          /* sy_sample_workspace bytes, 16-byte aligned, or NULL if 0 */
-  int64_t workspace_bytes;
+  void* workspace;          /* not used: NULL */
+  int64_t workspace_bytes;  /* not used: 0 */
   int64_t rows, vocab, logits_row;
   int32_t dtype;
 } sy_sample_args;
 
-/* Bytes of workspace sy_sample needs for these sizes, or -status. */
+/* 0: sy_sample needs no workspace; or -status where it would refuse the sizes.
+ * Needs no device. */
 SY_API int64_t sy_sample_workspace(const sy_sample_args* args);
 
 /*

@@ -4,7 +4,7 @@ from __future__ import annotations
 
 import ctypes
 
-from test_serving_cpu import Attend
+from test_serving_cpu import Attend, Sample
 
 
 def test_strides_of_the_abi():
@@ -27,3 +27,13 @@ def test_scale_times_log2_e_must_be_finite():
     nothing = dict(q_len=1, q_heads=2, kv_heads=1, head_dim=64, pages=4, page_size=16)
     for scale, want in ((2.3e38, N.SY_OK), (2.4e38, N.SY_ERR_ARG), (2.9e38, N.SY_ERR_ARG)):
         assert N.lib.sy_attend(ctypes.byref(Attend(batch=0, scale=scale, **nothing)), None) == want, scale
+
+
+def test_sampling_needs_no_workspace():
+    from switchyard import _native as N
+
+    def need(**kw):
+        return N.lib.sy_sample_workspace(ctypes.byref(Sample(**{**dict(rows=64, vocab=32000, logits_row=32000), **kw})))
+
+    assert need() == 0 and need(rows=0) == 0
+    assert need(vocab=0) == -N.SY_ERR_ARG and need(dtype=9) == -N.SY_ERR_DTYPE
