@@ -126,8 +126,8 @@ def generate(
     it they come from ``generator``. The sampling parameters are
     :func:`~switchyard.sample_tokens`'s. Returns the tokens ``[n_samples, max_new]``
     and their log-probabilities under the distribution they were drawn from. A
-    sample that meets logits with nothing to draw from (all NaN after an overflow,
-    say) ends there: its tokens are -1 and its log-probabilities NaN from then on.
+    sample that meets logits with nothing to draw from (all NaN after an overflow)
+    ends there: its tokens are -1 and its log-probabilities NaN from then on.
     One host synchronisation at most, when the caller reads the result.
     """
     cfg = model.cfg

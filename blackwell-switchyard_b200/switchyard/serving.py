@@ -118,7 +118,8 @@ def sample_tokens(
     their sum. ``temperature <= 0`` takes the highest logit. Weights are whole
     numbers, ``exp(x - max)`` in units of 2^-40, so the result does not depend
     on any order of summation and repeats bit for bit. NaN counts as ``-inf``;
-    a row with nothing above ``-inf`` gives token -1.
+    a row with no ``x`` above ``-inf`` gives token -1 (so does one whose products
+    all overflow, e.g. the type's lowest value at a temperature below 1).
 
     Returns int64 tokens ``[rows]``, or ``(tokens, logprob)`` with the fp32
     logarithm of the token's share of the kept weight.

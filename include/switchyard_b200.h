@@ -407,8 +407,9 @@ SY_API int64_t sy_sample_workspace(const sy_sample_args* args);
  * ceil(top_p Z), the first always; of those the ones with exp(x_i - max x) >=
  * min(min_p, 1). The token is the first in index order whose inclusive kept
  * weight exceeds floor(u Z_kept); logprob = log(w_token / Z_kept).
- * temperature <= 0 takes the highest logit. A row without a logit above -inf
- * gives token -1 and logprob NaN.
+ * temperature <= 0 takes the highest logit. A row without an x above -inf
+ * gives token -1 and logprob NaN (also where every logit times 1 / temperature
+ * overflows to -inf, as the type's lowest value does below temperature 1).
  */
 SY_API int sy_sample(const sy_sample_args* args, sy_stream_t stream);
 
