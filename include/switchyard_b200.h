@@ -359,8 +359,17 @@ typedef struct sy_attend_args {
   int32_t dtype; /* SY_BF16 or SY_F16 */
 } sy_attend_args;
 
-/* Bytes of workspace sy_attend needs for these sizes (pointers are not read),
- * or -status. */
+/*
+ * Bytes of workspace sy_attend needs for these sizes (pointers are not read), or
+ * -status. Partial rows take it: with R = q_len * q_heads / kv_heads rows per
+ * sequence and key head, L = 4 * (head_dim <= 64 ? 66 : 130) bytes a row,
+ *   R <= 128:  2 (batch * kv_heads + SMs) R L, and with a shared prefix (batch > 1)
+ *              2 (kv_heads * ceil(batch R / 256) + SMs) min(128, batch R) L more;
+ *   R > 128:   512 SMs L
+ * and 4 bytes per sequence and 256 rows. For single tokens that is small (128
+ * sequences of 32 / 8 heads of 128: 5 MB, 27 MB with a prefix); for 1024
+ * sequences of 8 key heads with 128 rows each it is 1.1 GB.
+ */
 SY_API int64_t sy_attend_workspace(const sy_attend_args* args);
 
 /*

@@ -218,3 +218,32 @@ def test_attend_what_stands_in_for_indices_outside(sy):
     out, lse = sy.attend_paged(q, kc, vc, table, torch.stack([lens[0], -lens[1]]), **kw, return_lse=True)
     assert _native.device_error() == 4
     check_attend(out, lse, args, kw, lead, [[side[0], side[1][:, :0]] for side in own])
+
+
+# ---------------------------------------------------------------------------
+# what the header says of workspaces
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("batch,n,hq,hk,d,width,prefix", [
+    (1, 1, 16, 16, 128, 33, 0), (128, 1, 32, 8, 128, 8, 16384), (24, 5, 24, 8, 64, 11, 1999), (1, 4096, 16, 16, 128, 64, 0),
+    (1024, 8, 128, 8, 128, 16, 0), (3, 129, 4, 4, 80, 16, 50),
+])
+def test_attend_workspace_is_as_documented(batch, n, hq, hk, d, width, prefix):
+    import ctypes
+
+    from switchyard import _native
+    from test_serving_cpu import Attend
+
+    args = Attend(batch=batch, q_len=n, q_heads=hq, kv_heads=hk, head_dim=d, pages=99, page_size=64,
+                  table_width=width, table_row=width, prefix_len=prefix, scale=1.0)
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    rows, line = n * (hq // hk), 4 * (2 + (64 if d <= 64 else 128))
+    wide = rows > 128
+    shared = prefix > 0 and batch > 1 and not wide
+    most = (4 * sms * 128 if wide else 2 * (batch * hk + sms) * rows) * line
+    if shared:
+        most += 2 * (hk * -(-batch * rows // 256) + sms) * min(128, batch * rows) * line
+    most += 4 * (batch * -(-rows // 256) + 1)
+    got = _native.lib.sy_attend_workspace(ctypes.byref(args))
+    assert most <= got <= most + 5 * 16
