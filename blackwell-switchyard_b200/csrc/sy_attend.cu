@@ -32,11 +32,11 @@
 // with its own O and (m, l).
 //
 // What bounds it (B200, bf16, head_dim 128). Few rows a sequence: DRAM; four
-// sequences of up to 65536 keys take 92 us, 0.87 of the measured copy rate, with
-// the join 0.78. Many rows: a step's scores wait for P V two steps back, as two
-// score buffers a stream are what 512 TMEM columns hold beside two outputs; a
-// prompt of 4096 tokens takes 102 us and 16 us of joining, 590 TFLOP/s, with the
-// tensor pipe and the exponentials each 38 % busy.
+// sequences of up to 65536 keys take 93 us, 0.88 of the measured copy rate, with
+// the 8 us of the join 0.81. Many rows: a step's scores wait for P V two steps
+// back, as two score buffers a stream are what 512 TMEM columns hold beside two
+// outputs; a prompt of 4096 tokens takes 107 us and 16 us of joining, 565 TFLOP/s
+// over both, with the tensor pipe 37 % and the exponentials 38 % busy.
 #include <cmath>
 
 #include "sy_common.cuh"
@@ -513,7 +513,13 @@ __device__ __forceinline__ float row_max(const uint32_t* x) {
   return fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3]));
 }
 
-// 32 weights 2^(c x + off) from x[0..31]: summed, then rounded to 16 bits into x[0..15]
+// 32 weights 2^(c x + off) from x[0..31]: summed, then rounded to 16 bits into x[0..15].
+// The rounding is the tensor cores' price: an MMA takes P and V in one type, and
+// 32-bit weights would be two 16-bit parts and twice the MMAs of P V. It adds about
+// as much as the output's own rounding: against 64 bits bf16 outputs are off by
+// 1.9e-3 to 2.3e-3 of their size where 32-bit weights give 1.6e-3 to 1.7e-3, fp16
+// by 2.8e-4 against 2.1e-4. The sums are of the unrounded weights, so lse keeps
+// 32 bits.
 template <typename T>
 __device__ __forceinline__ void weights(uint32_t* x, float c, float off, float2& sum0, float2& sum1) {
   const float2 c2 = make_float2(c, c), off2 = make_float2(off, off);

@@ -17,8 +17,11 @@
 // The draw then adds the kept weights in index order: CTAs, warps, lanes.
 //
 // The row's bytes are the floor for many rows (256 x 131071 fp32: 20.5 us at the
-// measured copy rate; 244 us, half of the issue slots and about 33 rows in flight);
-// for one row it is a chain of six to nine cluster barriers.
+// measured copy rate; 246 us, 44 % of the issue slots and about 37 rows in flight);
+// for few rows (1 x 32000: 18 us) it is a chain of cluster barriers: three without
+// top_k and top_p or for one token, seven with one of them or with both cuts in
+// one bin, nine with the cuts in two, two more where the bins next to the maximum
+// do not hold the cut, and 32 for each cut made by radix passes.
 // A remote shared-memory read costs as much as a barrier, so CTAs push what others
 // need (maxima, sums, the leader's verdicts) ahead of the barrier and read locally.
 #include <cooperative_groups.h>
